@@ -355,6 +355,111 @@ int moddit_refresh_merge(const void* prev, const void* cur, const uint8_t* mask,
                          int64_t mask_head_stride, int64_t mask_row_stride,
                          int heads, int n, void* out, moddit_stream_t stream);
 
+/*
+ * Gradients of moddit_flash_fwd at q, k and v, from its output o, its lse, the gradient grad_o of
+ * the output and, unless NULL, the gradient grad_lse of the LSE (both fp32 contiguous (B,H,q_len)):
+ *   P = exp(scale q.k - lse), delta = sum_d grad_o o - grad_lse, dS = P (grad_o.v - delta),
+ *   dq = scale dS k, dk = scale dS^T q, dv = P^T grad_o
+ * in fp32 with P and dS rounded to the storage type (fp16: held at powers of two that keep
+ * them in its range), each output rounded once. Rows with lse = -inf attend to nothing: they get
+ * dq = 0 and add nothing. Sums are formed in a fixed order: results repeat bit for bit.
+ * q_len or kv_len may be 0 (the other side's gradients are then zeros). batch * heads <= 65535.
+ * `workspace`: moddit_attention_bwd_workspace_bytes bytes, 16-byte aligned, one per call in
+ * flight. No gradient may overlap an input.
+ */
+int64_t moddit_attention_bwd_workspace_bytes(int batch, int heads, int q_len, int kv_len,
+                                             int head_dim, int dtype, int grid_origin);
+int moddit_flash_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse,
+                     const void* grad_o, const float* grad_lse, void* dq, void* dk, void* dv,
+                     int batch, int heads, int q_len, int kv_len, int head_dim,
+                     const int64_t q_strides[3], const int64_t k_strides[3],
+                     const int64_t v_strides[3], const int64_t o_strides[3],
+                     const int64_t go_strides[3], const int64_t dq_strides[3],
+                     const int64_t dk_strides[3], const int64_t dv_strides[3], float softmax_scale,
+                     int dtype, void* workspace, int64_t workspace_bytes, moddit_stream_t stream);
+
+/*
+ * The same for moddit_block_sparse_fwd: (counts, entries) are the forward's tile lists and
+ * (key_counts, key_entries) the same pairs by key tile, from moddit_transpose_tiles: for head h and
+ * the 128 grid keys of tile t < n_ktiles = ceil((kv_len - grid_origin) / 128) the query blocks of 64
+ * rows that attend to it, ascending, each as (query block << 2) | keys, bit 0 for keys 0..63 of the
+ * tile and bit 1 for keys 64..127.
+ */
+int moddit_block_sparse_bwd(const void* q, const void* k, const void* v, const void* o,
+                            const float* lse, const void* grad_o, const float* grad_lse, void* dq,
+                            void* dk, void* dv, int batch, int heads, int q_len, int kv_len,
+                            int head_dim, const int64_t q_strides[3], const int64_t k_strides[3],
+                            const int64_t v_strides[3], const int64_t o_strides[3],
+                            const int64_t go_strides[3], const int64_t dq_strides[3],
+                            const int64_t dk_strides[3], const int64_t dv_strides[3],
+                            float softmax_scale, int dtype, const int32_t* counts,
+                            const int32_t* entries, int n_qtiles, int cap,
+                            const int32_t* key_counts, const int32_t* key_entries, int n_ktiles,
+                            int key_cap, int grid_origin, void* workspace, int64_t workspace_bytes,
+                            moddit_stream_t stream);
+
+/*
+ * Tile lists by key tile (see moddit_block_sparse_bwd) of the lists (counts, entries) of
+ * moddit_block_sparse_fwd, whose key tiles ascend. Entries of key tiles from 2 * n_ktiles on are
+ * dropped. key_counts (heads, n_ktiles), key_entries (heads, n_ktiles, key_cap), key_cap =
+ * 2 * n_qtiles; n_qtiles <= 6144.
+ */
+int moddit_transpose_tiles(const int32_t* counts, const int32_t* entries, int heads, int n_qtiles,
+                           int cap, int32_t* key_counts, int32_t* key_entries, int n_ktiles,
+                           int key_cap, moddit_stream_t stream);
+
+/* Norms of moddit_qk_norm_rope. */
+enum moddit_norm { MODDIT_NORM_NONE = 0, MODDIT_NORM_RMS = 1, MODDIT_NORM_LAYER = 2 };
+
+/*
+ * Norm of queries and keys and the rotation of their positions, in one pass.
+ *   x^ = x r,         r = 1 / sqrt(mean(x^2) + eps)              MODDIT_NORM_RMS
+ *   x^ = (x - mu) r,  r = 1 / sqrt(mean((x - mu)^2) + eps)       MODDIT_NORM_LAYER
+ * over a head's D values, or with across_heads over the heads*D values of a token (at most
+ * 8192), then y = x^ * weight + bias (each may be NULL; D values, or heads*D with across_heads,
+ * of weight_dtype), and for the tokens [rope_offset, rope_offset + rope_len) each pair (a, c) of
+ * a head turned by its angle: (a cos - c sin, c cos + a sin). Pairs are elements (2i, 2i+1) with
+ * `interleaved`, else (i, i + D/2). Row t - rope_offset of the fp32 tables cos / sin, at
+ * b * table_strides[0] + row * table_strides[1] elements, holds table_dim = D/2 values, one a
+ * pair, or D: a pair's cos is then read at its first element and its sin at its second.
+ * q (batch, heads, q_len, D) and k (batch, heads, k_len, D): bf16 or fp16, D in {64,128}; the
+ * rotated tokens lie inside both. Arithmetic is fp32, rounded once. An output may be its own
+ * input (same pointer and strides); other overlaps are not allowed.
+ * Replaces the processors' norm_q / norm_k and apply_rotary_emb
+ * (MoD/models/wan/attention_processor.py:60-90, hunyuan/attention_processor.py:40-108,
+ * cogvideox/attention_processor.py:89-135).
+ */
+int moddit_qk_norm_rope(const void* q, const void* k, void* q_out, void* k_out, int batch, int heads,
+                        int q_len, int k_len, int head_dim, const int64_t q_strides[3],
+                        const int64_t k_strides[3], const int64_t qo_strides[3],
+                        const int64_t ko_strides[3], int dtype, int norm, int across_heads, float eps,
+                        const void* q_weight, const void* k_weight, const void* q_bias,
+                        const void* k_bias, int weight_dtype, const float* cos, const float* sin,
+                        const int64_t table_strides[2], int table_dim, int rope_offset, int rope_len,
+                        int interleaved, moddit_stream_t stream);
+
+/*
+ * Gradients of moddit_qk_norm_rope at its inputs q, k for the gradients dq_out, dk_out of its
+ * outputs: dq, dk in the storage type (a dq may be its own dq_out), and fp32 sums over batch,
+ * (heads) and tokens for weights and biases, each NULL where it is not wanted. With
+ * MODDIT_NORM_NONE q and k are not read and may be NULL. Where a weight's or bias's gradient is
+ * wanted, `workspace` holds the partial sums, added in a fixed order: at least
+ * moddit_qk_norm_rope_bwd_workspace_floats floats. A call without tokens writes nothing.
+ */
+int64_t moddit_qk_norm_rope_bwd_workspace_floats(int batch, int heads, int q_len, int k_len,
+                                                 int head_dim, int across_heads);
+int moddit_qk_norm_rope_bwd(const void* q, const void* k, const void* dq_out, const void* dk_out,
+                            void* dq, void* dk, float* dq_weight, float* dk_weight, float* dq_bias,
+                            float* dk_bias, int batch, int heads, int q_len, int k_len, int head_dim,
+                            const int64_t q_strides[3], const int64_t k_strides[3],
+                            const int64_t dqo_strides[3], const int64_t dko_strides[3],
+                            const int64_t dq_strides[3], const int64_t dk_strides[3], int dtype,
+                            int norm, int across_heads, float eps, const void* q_weight,
+                            const void* k_weight, int weight_dtype, const float* cos,
+                            const float* sin, const int64_t table_strides[2], int table_dim,
+                            int rope_offset, int rope_len, int interleaved, float* workspace,
+                            int64_t workspace_floats, moddit_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,6 +17,7 @@ MODDIT_EUNSUPPORTED = 2
 MODDIT_EHIP = 3
 
 BF16, FP16, FP32 = 0, 1, 2
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
 MODE_SPARSE, MODE_BLOCK_DIAGONAL, MODE_FULL = 0, 1, 2
 LAYOUT_WAN, LAYOUT_HUNYUAN, LAYOUT_COGVIDEOX, LAYOUT_OTHER = 0, 1, 2, 3
 
@@ -69,6 +70,17 @@ _SIGNATURES = {
                                     _vp, _vp, _vp, _i, _i, _vp]),
     "moddit_mask_to_tiles": (_i, [_vp, _i, _i, _i, ctypes.c_int64, ctypes.c_int64, _i, _i, _i,
                                   _vp, _vp, _i, _i, _vp]),
+    "moddit_attention_bwd_workspace_bytes": (ctypes.c_int64, [_i] * 7),
+    "moddit_flash_bwd": (_i, [_vp] * 10 + [_i] * 5 + [_c_i64p] * 8 + [_f, _i, _vp, ctypes.c_int64, _vp]),
+    "moddit_block_sparse_bwd": (_i, [_vp] * 10 + [_i] * 5 + [_c_i64p] * 8 + [_f, _i] +
+                                [_vp, _vp, _i, _i] * 2 + [_i, _vp, ctypes.c_int64, _vp]),
+    "moddit_transpose_tiles": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _i, _i, _vp]),
+    "moddit_qk_norm_rope": (_i, [_vp] * 4 + [_i] * 5 + [_c_i64p] * 4 + [_i] * 3 + [_f] + [_vp] * 4 +
+                            [_i, _vp, _vp, _c_i64p] + [_i] * 4 + [_vp]),
+    "moddit_qk_norm_rope_bwd_workspace_floats": (ctypes.c_int64, [_i] * 6),
+    "moddit_qk_norm_rope_bwd": (_i, [_vp] * 10 + [_i] * 5 + [_c_i64p] * 6 + [_i] * 3 + [_f] +
+                                [_vp] * 2 + [_i, _vp, _vp, _c_i64p] + [_i] * 4 +
+                                [_vp, ctypes.c_int64, _vp]),
     "moddit_refresh_merge": (_i, [_vp, _vp, _vp, ctypes.c_int64, ctypes.c_int64, _i, _i,
                                   _vp, _vp]),
 }
@@ -112,7 +124,12 @@ def check(rc: int, what: str) -> None:
 
 
 _i64x3 = ctypes.c_int64 * 3
+_i64x2 = ctypes.c_int64 * 2
 
 
 def strides3(*vals: int):
     return _i64x3(*vals)
+
+
+def strides2(*vals: int):
+    return _i64x2(*vals)

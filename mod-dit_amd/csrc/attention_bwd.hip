@@ -1,0 +1,784 @@
+// Gradients of dense and block-sparse attention for gfx950.
+//
+// With s = scale Q.K, P = exp(s - LSE) (the forward's natural-log LSE), and for the gradients dO
+// of the output and dL of the LSE:
+//   delta_i = sum_d dO_id O_id - dL_i
+//   dP = dO V^T,  dS = P (dP - delta),  dV = P^T dO,  dQ = scale dS K,  dK = scale dS^T Q.
+// A (row, key) pair takes 10 D FLOP. P is computed again from Q, K and the LSE: nothing of the
+// size of P is kept.
+//
+// Two passes of one kernel body. Each workgroup owns 128 rows of one side and streams tiles of 64
+// rows of the other: the dQ pass owns queries and streams keys, the dK/dV pass owns keys and
+// streams queries, so every sum stays in one workgroup's registers: no atomics, and results do
+// not depend on the order of workgroups. The price is that S and dP are computed twice, 14 D FLOP
+// a pair; adding dQ's parts across workgroups instead would take 4 D bytes of atomics per row and
+// 128 keys, more time than the products (2 D 128 FLOP each), in an order that changes.
+//
+// As in the forward the products are transposed: streamed rows are the A operand and owned rows
+// the columns, on MFMA 16x16x32. The accumulators of S and dP (streamed 4g + j, owned c16) are
+// then the B operand of the sums dQ^T += K^T dS^T, dV^T += dO^T P, dK^T += Q^T dS, so P and dS never
+// leave registers; their A operands come out of the same row-major tiles through
+// ds_read_b64_tr_b16.
+//
+// Rows of the grid outside the sequence: streamed ones load zeros; as queries they have
+// -LSE = -inf, so P = 0, as keys their scores are set to -inf. A query without keys has LSE = -inf
+// and adds nothing. Owned ones load a clamped row and store nothing.
+//
+// fp16 holds 2^-24 to 65504: P is rounded as 2^15 P, and dS as 2^e dS with the largest e for
+// which the head's largest |dO| (|V| + |O|) + |dL| stays below 2^14; bf16 needs neither.
+#include "common.h"
+#include "lds_dma.h"
+
+#include <type_traits>
+
+namespace moddit {
+namespace {
+
+constexpr int kBM = 128;  // owned rows per workgroup
+constexpr int kBN = 64;   // streamed rows per tile
+constexpr int kThreads = 256;
+constexpr int kStatsBytes = 1024;  // one DMA window; a block's 64 -LSE and 64 -delta take half
+constexpr float kPExponent = 15.f;  // fp16: P is held as 2^15 P
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ s16x4 lds_read_tr16(const unsigned char* a) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a));
+}
+
+template <int D>
+struct BwdLds {
+  static constexpr int kRowBytes = D * 2;
+  static constexpr int kTileBytes = kBN * kRowBytes;
+  static constexpr int kRowsPerWindow = 1024 / kRowBytes;
+  static constexpr int kWinPerWave = kTileBytes / 1024 / 4;
+  static constexpr int kStage = 2 * kTileBytes + kStatsBytes;
+  static constexpr int kTotal = 2 * kStage;
+};
+
+// XOR on the 16-byte chunks of LDS row r. Both reads of a tile are free of bank conflicts: the
+// 16 rows of a row read lie in 16 different chunks of 256 bytes, and so do the 8 rows x 2 chunks
+// of a half wave's transposed read.
+template <int D>
+__device__ __forceinline__ int swz(int r) {
+  return D == 128 ? 2 * (r & 7) + ((r >> 3) & 1) : 2 * ((r >> 1) & 3) + ((r >> 3) & 1);
+}
+
+struct RowsOf {
+  const uint16_t* p;
+  int64_t sb, sh, ss;
+};
+
+struct BwdParams {
+  RowsOf own1, own2;  // Q, dO (dQ pass) or K, V (dK/dV pass)
+  RowsOf str1, str2;  // K, V or Q, dO
+  uint16_t* out1;     // dQ or dK
+  uint16_t* out2;     // dV
+  int64_t o1_sb, o1_sh, o1_ss;
+  int64_t o2_sb, o2_sh, o2_ss;
+  int heads;
+  int own_len, str_len;
+  int origin;
+  int n_tiles;      // tiles of 128 owned rows
+  int n_str_tiles;  // tiles of 64 streamed rows
+  int xcd_run;
+  uint32_t str1_bytes, str2_bytes;  // span of one head's streamed rows
+  float scale, scale_log2;
+  const float* stats;  // [b,h][block of 64 grid rows][64 -LSE log2 units, 64 -delta]
+  int stat_blocks;
+  const float* maxima;  // fp16: [b,h][n_maxima][4], see stats_kernel
+  int n_maxima;
+  const int32_t* counts;
+  const int32_t* entries;
+  int cap;
+};
+
+// ---- row statistics ----
+struct StatsParams {
+  RowsOf o, d, v;
+  const float* lse;
+  const float* dlse;  // may be null
+  float* stats;
+  float* maxima;
+  int heads;
+  int q_len, kv_len;
+  int origin;
+  int stat_blocks;
+  int n_maxima;
+  float p_exponent;
+};
+
+// Block i of a head: -LSE (log2 units, with the exponent that P is held at) and -delta of the 64
+// grid rows from 64 i on; with kMax also the largest finite |dO|^2, |O|^2, |V|^2 and |dL| of its rows.
+// Reads O, dO (and V) once: bound by HBM.
+template <int D, typename E, bool kMax>
+__global__ __launch_bounds__(kThreads) void stats_kernel(StatsParams p) {
+  constexpr int kLanes = D / 8;
+  constexpr int kRows = kThreads / kLanes;
+  __shared__ float red[4][4];
+  const int bh = blockIdx.y;
+  const int b = bh / p.heads, h = bh % p.heads;
+  const int blk = blockIdx.x;
+  const int l = threadIdx.x % kLanes;
+  float top[4] = {0.f, 0.f, 0.f, 0.f};
+  // a row that is not finite spoils what it reaches whatever the scale, and must not set the others'
+  auto finite_max = [](float m, float x) { return x < INFINITY ? fmaxf(m, x) : m; };
+  auto row_sum = [](float x) {
+#pragma unroll
+    for (int m = 1; m < kLanes; m *= 2) x += __shfl_xor(x, m);
+    return x;
+  };
+#pragma unroll
+  for (int i = 0; i < 64 / kRows; ++i) {
+    const int r = i * kRows + threadIdx.x / kLanes;
+    if (blk < p.stat_blocks) {
+      const int token = p.origin + blk * 64 + r;
+      const bool in = token >= 0 && token < p.q_len;
+      u32x4 o = u32x4{0, 0, 0, 0}, d = o;
+      if (in) {
+        o = reinterpret_cast<const u32x4*>(p.o.p + b * p.o.sb + h * p.o.sh + token * p.o.ss)[l];
+        d = reinterpret_cast<const u32x4*>(p.d.p + b * p.d.sb + h * p.d.sh + token * p.d.ss)[l];
+      }
+      float dot = 0.f, oo = 0.f, dd = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = E::to_float(u16_at(o, e)), y = E::to_float(u16_at(d, e));
+        dot += x * y;
+        if (kMax) {
+          oo += x * x;
+          dd += y * y;
+        }
+      }
+      dot = row_sum(dot);
+      float g = 0.f, nl = -INFINITY;
+      if (in) {
+        const int64_t at = static_cast<int64_t>(bh) * p.q_len + token;
+        const float lse = p.lse[at];
+        if (p.dlse != nullptr) g = p.dlse[at];
+        nl = lse == -INFINITY ? -INFINITY : p.p_exponent - lse * 1.4426950408889634f;
+      }
+      if (kMax) {
+        top[0] = finite_max(top[0], row_sum(dd));
+        top[1] = finite_max(top[1], row_sum(oo));
+        top[3] = finite_max(top[3], fabsf(g));
+      }
+      if (l == 0) {
+        float* s = p.stats + (static_cast<int64_t>(bh) * p.stat_blocks + blk) * 128;
+        s[r] = nl;
+        s[64 + r] = in ? g - dot : 0.f;
+      }
+    }
+    if (kMax) {
+      const int key = blk * 64 + r;
+      u32x4 v = u32x4{0, 0, 0, 0};
+      if (key < p.kv_len) v = reinterpret_cast<const u32x4*>(p.v.p + b * p.v.sb + h * p.v.sh + key * p.v.ss)[l];
+      float vv = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = E::to_float(u16_at(v, e));
+        vv += x * x;
+      }
+      top[2] = finite_max(top[2], row_sum(vv));
+    }
+  }
+  if constexpr (kMax) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int m = kLanes; m < 64; m *= 2) top[i] = fmaxf(top[i], __shfl_xor(top[i], m));
+      if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][i] = top[i];
+    }
+    __syncthreads();
+    if (threadIdx.x < 4)
+      p.maxima[(static_cast<int64_t>(bh) * p.n_maxima + blk) * 4 + threadIdx.x] =
+          fmaxf(fmaxf(red[0][threadIdx.x], red[1][threadIdx.x]), fmaxf(red[2][threadIdx.x], red[3][threadIdx.x]));
+  }
+}
+
+// The exponent e that fp16 dS is held at: the largest with 2^e (|dO| (|V| + |O|) + |dL|) < 2^14
+// over the head's finite rows and keys, so that |2^e dS| < 2^14 whatever P (which is at most 1, but
+// for rounding). 0 where the bound is 0. Every thread returns it.
+__device__ __forceinline__ int ds_exponent(const float* maxima, int n, float (*red)[4]) {
+  float top[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = threadIdx.x; i < n; i += kThreads)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], maxima[4 * i + k]);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) top[k] = fmaxf(top[k], __shfl_xor(top[k], m));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][k] = top[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 4; ++k) top[k] = fmaxf(fmaxf(red[0][k], red[1][k]), fmaxf(red[2][k], red[3][k]));
+  __syncthreads();
+  const float bound = sqrtf(top[0]) * (sqrtf(top[1]) + sqrtf(top[2])) + top[3];
+  if (!(bound > 0.f)) return 0;
+  int e;
+  frexpf(bound, &e);  // bound < 2^e
+  e = 14 - e;
+  return e < -100 ? -100 : (e > 100 ? 100 : e);
+}
+
+template <int D, typename E, bool kKeys, bool kSparse>
+__global__ __launch_bounds__(kThreads, D == 128 && kKeys ? 1 : 2) void attention_bwd_kernel(BwdParams p) {
+  using L = BwdLds<D>;
+  using V8 = typename E::vec8;
+  constexpr int kKC = D / 32;  // MFMA k-steps over d
+  constexpr int kDB = D / 16;  // 16-row blocks of the transposed sums
+  constexpr bool kHalf = std::is_same<E, Fp16>::value;
+
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int tid = threadIdx.x;
+  const int wave = tid >> 6;
+  const int lane = tid & 63;
+  const int g = lane >> 4;
+  const int c16 = lane & 15;
+
+  const int tile = xcd_remap(blockIdx.x, gridDim.x, p.xcd_run);
+  const int ot = tile % p.n_tiles;
+  const int bh = tile / p.n_tiles;
+  const int b = bh / p.heads;
+  const int h = bh - b * p.heads;
+
+  int n_iter = p.n_str_tiles;
+  const int32_t* list = nullptr;
+  if (kSparse) {
+    const int64_t slot = static_cast<int64_t>(h) * p.n_tiles + ot;
+    n_iter = p.counts[slot];
+    n_iter = n_iter < 0 ? 0 : (n_iter < p.cap ? n_iter : p.cap);
+    list = p.entries + slot * p.cap;
+  }
+  const int first_row = p.origin + ot * kBM + __builtin_amdgcn_readfirstlane(wave) * 32;
+  const int wbit = first_row < p.own_len && first_row + 31 >= 0 ? 1 << (wave >> 1) : 0;
+
+  float ds_scale = 1.f;  // fp16, dK/dV: 2^(e - 15), from 2^15 P to 2^e dS
+  float out1_scale = p.scale;
+  int ds_exp = 0;
+  if constexpr (kHalf) {
+    ds_exp = ds_exponent(p.maxima + static_cast<int64_t>(bh) * p.n_maxima * 4, p.n_maxima,
+                         reinterpret_cast<float(*)[4]>(smem));
+    ds_scale = ldexpf(1.f, ds_exp - static_cast<int>(kPExponent));
+    out1_scale *= ldexpf(1.f, -ds_exp);
+  }
+
+  // ---- owned rows (B operands): lane holds row 16qq + c16, dims 32c + 8g.. ----
+  const int row0 = p.origin + ot * kBM + wave * 32 + c16;
+  V8 own1[2][kKC], own2[2][kKC];
+#pragma unroll
+  for (int qq = 0; qq < 2; ++qq) {
+    const int row = row0 + 16 * qq;
+    const int r = row < 0 ? 0 : (row < p.own_len ? row : p.own_len - 1);
+    const u32x4* a = reinterpret_cast<const u32x4*>(p.own1.p + b * p.own1.sb + h * p.own1.sh + r * p.own1.ss);
+    const u32x4* c = reinterpret_cast<const u32x4*>(p.own2.p + b * p.own2.sb + h * p.own2.sh + r * p.own2.ss);
+#pragma unroll
+    for (int i = 0; i < kKC; ++i) {
+      own1[qq][i] = as_vec8<V8>(a[4 * i + g]);
+      own2[qq][i] = as_vec8<V8>(c[4 * i + g]);
+    }
+  }
+  const float* stats = p.stats + static_cast<int64_t>(bh) * p.stat_blocks * 128;
+  float nl_own[2] = {0.f, 0.f}, nd_own[2] = {0.f, 0.f};
+  if constexpr (!kKeys) {
+#pragma unroll
+    for (int qq = 0; qq < 2; ++qq) {
+      const int gr = ot * kBM + wave * 32 + 16 * qq + c16;
+      const float* s = stats + (gr >> 6) * 128 + (gr & 63);
+      nl_own[qq] = s[0] + (kHalf ? ds_exp - kPExponent : 0.f);
+      nd_own[qq] = s[64];
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0);
+
+  // ---- staging, as in the forward: window w of a tile holds LDS bytes [1024 w, +1024) ----
+  const u32x4 rsrc1 = raw_rsrc(p.str1.p + b * p.str1.sb + h * p.str1.sh, p.str1_bytes);
+  const u32x4 rsrc2 = raw_rsrc(p.str2.p + b * p.str2.sb + h * p.str2.sh, p.str2_bytes);
+  const u32x4 rsrc_st = raw_rsrc(stats, static_cast<uint32_t>(p.stat_blocks) * 512u);
+  const uint32_t lds0 = lds_addr(smem);
+  uint32_t src1[L::kWinPerWave], src2[L::kWinPerWave];
+#pragma unroll
+  for (int i = 0; i < L::kWinPerWave; ++i) {
+    const int w = wave * L::kWinPerWave + i;
+    const int r = w * L::kRowsPerWindow + (lane * 16) / L::kRowBytes;
+    const int ch = (((lane * 16) % L::kRowBytes) / 16) ^ swz<D>(r);
+    // rows before token 0 wrap to offsets beyond every range the descriptors admit
+    src1[i] = static_cast<uint32_t>(((p.origin + r) * static_cast<int>(p.str1.ss) + ch * 8) * 2);
+    src2[i] = static_cast<uint32_t>(((p.origin + r) * static_cast<int>(p.str2.ss) + ch * 8) * 2);
+  }
+  const uint32_t step1 = static_cast<uint32_t>(kBN * p.str1.ss * 2);
+  const uint32_t step2 = static_cast<uint32_t>(kBN * p.str2.ss * 2);
+  auto dma = [&](int st, int stage) {
+    const uint32_t dst = lds0 + stage * L::kStage;
+#pragma unroll
+    for (int i = 0; i < L::kWinPerWave; ++i)
+      lds_dma16(rsrc1, dst + (wave * L::kWinPerWave + i) * 1024, src1[i] + st * step1, 0);
+#pragma unroll
+    for (int i = 0; i < L::kWinPerWave; ++i)
+      lds_dma16(rsrc2, dst + L::kTileBytes + (wave * L::kWinPerWave + i) * 1024, src2[i] + st * step2, 0);
+    if (kKeys && wave == 0) lds_dma16(rsrc_st, dst + 2 * L::kTileBytes, lane * 16 + st * 512, 0);
+  };
+
+  // ---- LDS operand addressing ----
+  uint32_t row_rd[kKC];  // A operand of S and dP: row 16sb + c16, logical chunk 4c + g
+#pragma unroll
+  for (int c = 0; c < kKC; ++c)
+    row_rd[c] = static_cast<uint32_t>(c16 * L::kRowBytes + (((4 * c + g) ^ swz<D>(c16)) * 16));
+  // A operand of the sums, transposed: see v_rd in attention.hip
+  const int tr_row = 4 * g + (c16 >> 2);
+  uint32_t tr_rd[kDB];
+#pragma unroll
+  for (int db = 0; db < kDB; ++db) {
+    const int d = db * 16 + 4 * (c16 & 3);
+    tr_rd[db] = static_cast<uint32_t>(tr_row * L::kRowBytes + (((d >> 3) ^ swz<D>(tr_row)) * 16) + (d & 7) * 2);
+  }
+
+  f32x4 acc1[kDB][2], acc2[kKeys ? kDB : 1][2];
+#pragma unroll
+  for (int db = 0; db < kDB; ++db) {
+    acc1[db][0] = acc1[db][1] = f32x4{};
+    if (kKeys) acc2[db][0] = acc2[db][1] = f32x4{};
+  }
+
+  auto decode = [&](int e_raw, int& st, int& flags) {
+    const int e = __builtin_amdgcn_readfirstlane(e_raw);
+    st = e >> 2;
+    flags = (st >= 0 && st < p.n_str_tiles) ? (e & 3) : 0;  // as in the forward
+    st = st < 0 ? 0 : (st < p.n_str_tiles ? st : p.n_str_tiles - 1);
+  };
+  auto entry = [&](int i) -> int { return kSparse ? list[i] : ((i << 2) | 3); };
+  auto tr_operand = [&](const unsigned char* a) -> V8 {
+    const s16x4 lo = lds_read_tr16(a);
+    const s16x4 hi = lds_read_tr16(a + 16 * L::kRowBytes);
+    return as_vec8<V8>(u32x4{__builtin_bit_cast(u32x2, lo).x, __builtin_bit_cast(u32x2, lo).y,
+                             __builtin_bit_cast(u32x2, hi).x, __builtin_bit_cast(u32x2, hi).y});
+  };
+
+  // 32 streamed rows (half t of the tile) against the wave's 32 owned ones
+  auto half_tile = [&](const unsigned char* t1, const unsigned char* t2, const float* stt, int t, int st) {
+    f32x4 s[2][2], dp[2][2], nl[2];
+#pragma unroll
+    for (int sb = 0; sb < 2; ++sb) {
+      f32x4 nd;
+      if constexpr (kKeys) {
+        nl[sb] = *reinterpret_cast<const f32x4*>(stt + 32 * t + 16 * sb + 4 * g);
+        nd = *reinterpret_cast<const f32x4*>(stt + 64 + 32 * t + 16 * sb + 4 * g);
+      }
+#pragma unroll
+      for (int qq = 0; qq < 2; ++qq) {
+        s[sb][qq] = f32x4{};
+        dp[sb][qq] = kKeys ? nd : f32x4{nd_own[qq], nd_own[qq], nd_own[qq], nd_own[qq]};
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < kKC; ++c)
+#pragma unroll
+      for (int sb = 0; sb < 2; ++sb) {
+        const V8 a = *reinterpret_cast<const V8*>(t1 + row_rd[c] + (32 * t + 16 * sb) * L::kRowBytes);
+        s[sb][0] = E::mma16(a, own1[0][c], s[sb][0]);
+        s[sb][1] = E::mma16(a, own1[1][c], s[sb][1]);
+      }
+#pragma unroll
+    for (int c = 0; c < kKC; ++c)
+#pragma unroll
+      for (int sb = 0; sb < 2; ++sb) {
+        const V8 a = *reinterpret_cast<const V8*>(t2 + row_rd[c] + (32 * t + 16 * sb) * L::kRowBytes);
+        dp[sb][0] = E::mma16(a, own2[0][c], dp[sb][0]);
+        dp[sb][1] = E::mma16(a, own2[1][c], dp[sb][1]);
+      }
+    if constexpr (!kKeys) {
+      const int key0 = p.origin + st * kBN;
+      if (key0 < 0 || key0 + kBN > p.str_len) {
+        const int lo = -key0 - 32 * t - 4 * g, hi = p.str_len - key0 - 32 * t - 4 * g;
+#pragma unroll
+        for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const bool out = 16 * sb + j < lo || 16 * sb + j >= hi;
+            s[sb][0][j] = out ? -INFINITY : s[sb][0][j];
+            s[sb][1][j] = out ? -INFINITY : s[sb][1][j];
+          }
+      }
+    }
+    V8 pb[2], db_[2];
+#pragma unroll
+    for (int qq = 0; qq < 2; ++qq)
+#pragma unroll
+      for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float w = __builtin_amdgcn_exp2f(
+              __builtin_fmaf(s[sb][qq][j], p.scale_log2, kKeys ? nl[sb][j] : nl_own[qq]));
+          // rounded to the storage type, the MFMA's operand: 2^-9 (bf16) or 2^-12 (fp16) of each
+          // weight, the same as the forward's P
+          if (kKeys) pb[qq][4 * sb + j] = static_cast<typename E::elem>(w);
+          const float x = kHalf && kKeys ? w * ds_scale : w;
+          db_[qq][4 * sb + j] = static_cast<typename E::elem>(x * dp[sb][qq][j]);
+        }
+#pragma unroll
+    for (int db = 0; db < kDB; ++db) {
+      const V8 a = tr_operand(t1 + tr_rd[db] + t * 32 * L::kRowBytes);
+      acc1[db][0] = E::mma16(a, db_[0], acc1[db][0]);
+      acc1[db][1] = E::mma16(a, db_[1], acc1[db][1]);
+      if constexpr (kKeys) {
+        const V8 c = tr_operand(t2 + tr_rd[db] + t * 32 * L::kRowBytes);
+        acc2[db][0] = E::mma16(c, pb[0], acc2[db][0]);
+        acc2[db][1] = E::mma16(c, pb[1], acc2[db][1]);
+      }
+    }
+  };
+
+  int st = 0, flags = 0;
+  if (n_iter > 0) {
+    decode(entry(0), st, flags);
+    dma(st, 0);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+  }
+  for (int j = 0; j < n_iter; ++j) {
+    int st1 = 0, flags1 = 0;
+    if (j + 1 < n_iter) {
+      decode(entry(j + 1), st1, flags1);
+      dma(st1, (j + 1) & 1);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    const unsigned char* t1 = smem + (j & 1) * L::kStage;
+    if (flags & wbit) {
+      half_tile(t1, t1 + L::kTileBytes, reinterpret_cast<const float*>(t1 + 2 * L::kTileBytes), 0, st);
+      half_tile(t1, t1 + L::kTileBytes, reinterpret_cast<const float*>(t1 + 2 * L::kTileBytes), 1, st);
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    st = st1;
+    flags = flags1;
+  }
+
+#pragma unroll
+  for (int qq = 0; qq < 2; ++qq) {
+    const int row = row0 + 16 * qq;
+    if (row < 0 || row >= p.own_len) continue;
+    uint16_t* o1 = p.out1 + b * p.o1_sb + h * p.o1_sh + row * p.o1_ss;
+#pragma unroll
+    for (int db = 0; db < kDB; ++db) {
+      const f32x4 x = acc1[db][qq] * out1_scale;
+      u32x2 w;
+      w.x = pack2(E::from_float(x[0]), E::from_float(x[1]));
+      w.y = pack2(E::from_float(x[2]), E::from_float(x[3]));
+      *reinterpret_cast<u32x2*>(o1 + db * 16 + 4 * g) = w;
+    }
+    if constexpr (kKeys) {
+      uint16_t* o2 = p.out2 + b * p.o2_sb + h * p.o2_sh + row * p.o2_ss;
+#pragma unroll
+      for (int db = 0; db < kDB; ++db) {
+        const f32x4 x = acc2[db][qq] * (kHalf ? 0x1p-15f : 1.f);
+        u32x2 w;
+        w.x = pack2(E::from_float(x[0]), E::from_float(x[1]));
+        w.y = pack2(E::from_float(x[2]), E::from_float(x[3]));
+        *reinterpret_cast<u32x2*>(o2 + db * 16 + 4 * g) = w;
+      }
+    }
+  }
+}
+
+template <int D, typename E, bool kKeys, bool kSparse>
+int launch_pass(const BwdParams& p, int batch, hipStream_t st) {
+  constexpr int kLds = BwdLds<D>::kTotal;
+  auto kernel = attention_bwd_kernel<D, E, kKeys, kSparse>;
+  static LaunchSetup once;
+  if (set_dynamic_lds_once(once, reinterpret_cast<const void*>(kernel), kLds) != hipSuccess) {
+    set_error("attention_bwd: cannot reserve %d bytes of LDS", kLds);
+    return MODDIT_EHIP;
+  }
+  const int64_t tiles = static_cast<int64_t>(batch) * p.heads * p.n_tiles;
+  if (tiles == 0) return MODDIT_OK;
+  if (tiles > 0x7fffffff) {
+    set_error("attention_bwd: too many tiles (%lld)", static_cast<long long>(tiles));
+    return MODDIT_EINVAL;
+  }
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles)), dim3(kThreads), kLds, st, p);
+  MODDIT_CHECK_LAUNCH("attention_bwd");
+  return MODDIT_OK;
+}
+
+template <int D, typename E>
+int launch_bwd(const StatsParams& sp, const BwdParams& dq, const BwdParams& dkv, int batch, hipStream_t st) {
+  constexpr bool kMax = std::is_same<E, Fp16>::value;
+  const int blocks = kMax ? sp.n_maxima : sp.stat_blocks;
+  if (blocks > 0) {
+    hipLaunchKernelGGL((stats_kernel<D, E, kMax>), dim3(blocks, batch * sp.heads), dim3(kThreads), 0, st, sp);
+    MODDIT_CHECK_LAUNCH("attention_bwd (row statistics)");
+  }
+  const bool sparse = dq.counts != nullptr;
+  if (const int rc = sparse ? launch_pass<D, E, false, true>(dq, batch, st) : launch_pass<D, E, false, false>(dq, batch, st)) return rc;
+  return sparse ? launch_pass<D, E, true, true>(dkv, batch, st) : launch_pass<D, E, true, false>(dkv, batch, st);
+}
+
+// Blocks of 64 grid rows (whole tiles of 128) and of maxima, and the floats of both.
+int64_t stat_blocks_of(int q_len, int origin) { return (static_cast<int64_t>(q_len) - origin + kBM - 1) / kBM * 2; }
+int64_t maxima_of(int q_len, int kv_len, int origin) {
+  const int64_t a = stat_blocks_of(q_len, origin), b = (static_cast<int64_t>(kv_len) + 63) / 64;
+  return a > b ? a : b;
+}
+int64_t bwd_workspace_floats(int batch, int heads, int q_len, int kv_len, int dtype, int origin) {
+  return static_cast<int64_t>(batch) * heads *
+         (stat_blocks_of(q_len, origin) * 128 + (dtype == MODDIT_FP16 ? maxima_of(q_len, kv_len, origin) * 4 : 0));
+}
+
+struct BwdArgs {
+  const void *q, *k, *v, *o, *d;
+  const float *lse, *dlse;
+  void *dq, *dk, *dv;
+  int batch, heads, q_len, kv_len, head_dim;
+  const int64_t *qs, *ks, *vs, *os, *ds, *dqs, *dks, *dvs;
+  float scale;
+  int dtype;
+  const int32_t *counts, *entries;
+  int n_qtiles, cap;
+  const int32_t *key_counts, *key_entries;
+  int n_ktiles, key_cap;
+  int origin;
+  void* workspace;
+  int64_t workspace_bytes;
+};
+
+RowsOf rows_of(const void* p, const int64_t* s) { return RowsOf{static_cast<const uint16_t*>(p), s[0], s[1], s[2]}; }
+
+int bwd_entry(const BwdArgs& a, moddit_stream_t stream) {
+  clear_error();
+  const int64_t* strides[8] = {a.qs, a.ks, a.vs, a.os, a.ds, a.dqs, a.dks, a.dvs};
+  for (const int64_t* s : strides) {
+    MODDIT_CHECK_ARG(s != nullptr, "attention_bwd: null stride array");
+    for (int j = 0; j < 3; ++j)
+      MODDIT_CHECK_ARG(s[j] >= 0 && s[j] % 8 == 0, "attention_bwd: strides must be non-negative multiples of 8 elements");
+  }
+  MODDIT_CHECK_ARG(a.scale > 0.f && std::isfinite(a.scale), "attention_bwd: softmax_scale must be positive");
+  MODDIT_CHECK_ARG(a.batch >= 0 && a.heads >= 0 && a.q_len >= 0 && a.kv_len >= 0, "attention_bwd: negative size");
+  if (a.head_dim != 64 && a.head_dim != 128) {
+    set_error("attention_bwd: head_dim must be 64 or 128, got %d", a.head_dim);
+    return MODDIT_EUNSUPPORTED;
+  }
+  if (a.dtype != MODDIT_BF16 && a.dtype != MODDIT_FP16) {
+    set_error("attention_bwd: dtype must be bf16 or fp16");
+    return MODDIT_EUNSUPPORTED;
+  }
+  MODDIT_CHECK_ARG(a.origin > -kBN && a.origin <= 0, "attention_bwd: grid_origin must be in (-64, 0], got %d", a.origin);
+  const bool sparse = a.counts != nullptr;
+  const int64_t nq = (static_cast<int64_t>(a.q_len) - a.origin + kBM - 1) / kBM;
+  const int64_t nk = (static_cast<int64_t>(a.kv_len) - a.origin + kBM - 1) / kBM;
+  if (sparse) {
+    MODDIT_CHECK_ARG(a.entries && a.key_counts && a.key_entries, "attention_bwd: tile lists missing");
+    MODDIT_CHECK_ARG(a.n_qtiles == nq, "attention_bwd: n_qtiles=%d but q_len=%d (grid origin %d) needs %lld", a.n_qtiles,
+                     a.q_len, a.origin, static_cast<long long>(nq));
+    MODDIT_CHECK_ARG(a.n_ktiles == nk, "attention_bwd: n_ktiles=%d but kv_len=%d (grid origin %d) needs %lld", a.n_ktiles,
+                     a.kv_len, a.origin, static_cast<long long>(nk));
+    MODDIT_CHECK_ARG(a.cap > 0 && a.key_cap > 0, "attention_bwd: cap must be positive");
+  }
+  if (a.batch == 0 || a.heads == 0 || (a.q_len == 0 && a.kv_len == 0)) return MODDIT_OK;
+  MODDIT_CHECK_ARG(static_cast<int64_t>(a.batch) * a.heads <= 65535, "attention_bwd: batch * heads exceeds 65535");
+  MODDIT_CHECK_ARG((a.q_len == 0 || (a.q && a.o && a.d && a.lse && a.dq)) && (a.kv_len == 0 || (a.k && a.v && a.dk && a.dv)),
+                   "attention_bwd: null tensor pointer");
+  const void* all[8] = {a.q, a.k, a.v, a.o, a.d, a.dq, a.dk, a.dv};
+  for (const void* t : all) MODDIT_CHECK_ARG(aligned16(t), "attention_bwd: tensors must be 16-byte aligned");
+  const int64_t need = bwd_workspace_floats(a.batch, a.heads, a.q_len, a.kv_len, a.dtype, a.origin) * 4;
+  MODDIT_CHECK_ARG((a.workspace != nullptr || need == 0) && aligned16(a.workspace) && a.workspace_bytes >= need,
+                   "attention_bwd: a 16-byte aligned workspace of %lld bytes is needed, got %lld",
+                   static_cast<long long>(need), static_cast<long long>(a.workspace_bytes));
+
+  // Streamed rows are addressed with 32-bit byte offsets, a whole tile past the last included.
+  auto span = [](int len, const int64_t* s, int dim) { return len > 0 ? (static_cast<int64_t>(len) - 1) * s[2] * 2 + dim * 2 : 0; };
+  const int64_t spans[4] = {span(a.q_len, a.qs, a.head_dim), span(a.q_len, a.ds, a.head_dim),
+                            span(a.kv_len, a.ks, a.head_dim), span(a.kv_len, a.vs, a.head_dim)};
+  const int64_t last[4] = {nq * kBM * a.qs[2] * 2, nq * kBM * a.ds[2] * 2, nk * kBM * a.ks[2] * 2, nk * kBM * a.vs[2] * 2};
+  for (int i = 0; i < 4; ++i)
+    if (spans[i] > 0x7fffffffLL || last[i] > 0x7fffffffLL) {
+      set_error("attention_bwd: one head's rows exceed 2 GiB of 32-bit offsets");
+      return MODDIT_EUNSUPPORTED;
+    }
+
+  StatsParams sp;
+  sp.o = rows_of(a.o, a.os);
+  sp.d = rows_of(a.d, a.ds);
+  sp.v = rows_of(a.v, a.vs);
+  sp.lse = a.lse;
+  sp.dlse = a.dlse;
+  sp.heads = a.heads;
+  sp.q_len = a.q_len;
+  sp.kv_len = a.kv_len;
+  sp.origin = a.origin;
+  sp.stat_blocks = static_cast<int>(stat_blocks_of(a.q_len, a.origin));
+  sp.n_maxima = static_cast<int>(maxima_of(a.q_len, a.kv_len, a.origin));
+  sp.stats = static_cast<float*>(a.workspace);
+  sp.maxima = sp.stats + static_cast<int64_t>(a.batch) * a.heads * sp.stat_blocks * 128;
+  sp.p_exponent = a.dtype == MODDIT_FP16 ? kPExponent : 0.f;
+
+  BwdParams p;
+  p.heads = a.heads;
+  p.origin = a.origin;
+  p.scale = a.scale;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.stats = sp.stats;
+  p.stat_blocks = sp.stat_blocks;
+  p.maxima = sp.maxima;
+  p.n_maxima = sp.n_maxima;
+  BwdParams dq = p, dkv = p;
+  dq.own1 = dkv.str1 = rows_of(a.q, a.qs);
+  dq.own2 = dkv.str2 = rows_of(a.d, a.ds);
+  dq.str1 = dkv.own1 = rows_of(a.k, a.ks);
+  dq.str2 = dkv.own2 = rows_of(a.v, a.vs);
+  dq.out1 = static_cast<uint16_t*>(a.dq);
+  dq.o1_sb = a.dqs[0]; dq.o1_sh = a.dqs[1]; dq.o1_ss = a.dqs[2];
+  dq.out2 = nullptr;
+  dq.o2_sb = dq.o2_sh = dq.o2_ss = 0;
+  dkv.out1 = static_cast<uint16_t*>(a.dk);
+  dkv.out2 = static_cast<uint16_t*>(a.dv);
+  dkv.o1_sb = a.dks[0]; dkv.o1_sh = a.dks[1]; dkv.o1_ss = a.dks[2];
+  dkv.o2_sb = a.dvs[0]; dkv.o2_sh = a.dvs[1]; dkv.o2_ss = a.dvs[2];
+  dq.own_len = dkv.str_len = a.q_len;
+  dq.str_len = dkv.own_len = a.kv_len;
+  dq.n_tiles = a.q_len > 0 ? static_cast<int>(nq) : 0;
+  dkv.n_tiles = a.kv_len > 0 ? static_cast<int>(nk) : 0;
+  dq.n_str_tiles = a.kv_len > 0 ? static_cast<int>((static_cast<int64_t>(a.kv_len) - a.origin + kBN - 1) / kBN) : 0;
+  dkv.n_str_tiles = a.q_len > 0 ? static_cast<int>((static_cast<int64_t>(a.q_len) - a.origin + kBN - 1) / kBN) : 0;
+  dq.xcd_run = xcd_run_for(static_cast<int64_t>(a.kv_len) * a.head_dim * 4);
+  dkv.xcd_run = xcd_run_for(static_cast<int64_t>(a.q_len) * a.head_dim * 4);
+  dkv.str1_bytes = static_cast<uint32_t>(spans[0]);
+  dkv.str2_bytes = static_cast<uint32_t>(spans[1]);
+  dq.str1_bytes = static_cast<uint32_t>(spans[2]);
+  dq.str2_bytes = static_cast<uint32_t>(spans[3]);
+  dq.counts = a.counts;
+  dq.entries = a.entries;
+  dq.cap = a.cap;
+  dkv.counts = a.key_counts;
+  dkv.entries = a.key_entries;
+  dkv.cap = a.key_cap;
+  // lists of a side whose counterpart is empty name no row
+  if (sparse && (a.q_len == 0 || a.kv_len == 0)) dq.counts = dkv.counts = nullptr;
+
+  hipStream_t st = as_stream(stream);
+  const bool bf = a.dtype == MODDIT_BF16;
+  if (a.head_dim == 128)
+    return bf ? launch_bwd<128, Bf16>(sp, dq, dkv, a.batch, st) : launch_bwd<128, Fp16>(sp, dq, dkv, a.batch, st);
+  return bf ? launch_bwd<64, Bf16>(sp, dq, dkv, a.batch, st) : launch_bwd<64, Fp16>(sp, dq, dkv, a.batch, st);
+}
+
+// ---- tile lists by key tile ----
+// Workgroup (head, 16 key tiles of 128): the bits (query block of 64 rows, key tile of 64) of its
+// 32 key tiles are set in LDS by threads that each walk their query tiles' lists (ascending, so a
+// binary search finds the part inside), then each wave writes the list of four key tile pairs,
+// 64 query blocks at a time.
+constexpr int kPairs = 16;
+constexpr int kMaxBlocks = 12288;  // query blocks a call: 32 rows of bits in 48 KB of LDS
+
+__global__ __launch_bounds__(kThreads) void transpose_tiles_kernel(const int32_t* counts, const int32_t* entries,
+                                                                  int n_qtiles, int cap, int n_pairs, int words,
+                                                                  int32_t* out_counts, int32_t* out_entries) {
+  extern __shared__ uint32_t bits[];  // [2 * kPairs][words]: bit b of word w is query block 32 w + b
+  const int h = blockIdx.y;
+  const int k0 = blockIdx.x * 2 * kPairs;
+  for (int i = threadIdx.x; i < 2 * kPairs * words; i += kThreads) bits[i] = 0;
+  __syncthreads();
+  for (int t = threadIdx.x; t < n_qtiles; t += kThreads) {
+    const int64_t slot = static_cast<int64_t>(h) * n_qtiles + t;
+    const int32_t* list = entries + slot * cap;
+    int n = counts[slot];
+    n = n < 0 ? 0 : (n < cap ? n : cap);
+    int lo = 0, hi = n;
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if ((list[mid] >> 2) < k0) lo = mid + 1; else hi = mid;
+    }
+    for (; lo < n; ++lo) {
+      const int e = list[lo], k = (e >> 2) - k0;
+      if (k < 0 || k >= 2 * kPairs) break;
+      if (e & 3) atomicOr(&bits[k * words + t / 16], static_cast<uint32_t>(e & 3) << (2 * (t % 16)));
+    }
+  }
+  __syncthreads();
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (int i = wave; i < kPairs; i += kThreads / 64) {
+    const int pair = blockIdx.x * kPairs + i;
+    if (pair >= n_pairs) break;
+    const int64_t slot = static_cast<int64_t>(h) * n_pairs + pair;
+    int32_t* list = out_entries + slot * 2 * n_qtiles;
+    int n = 0;
+    for (int b0 = 0; b0 < 2 * n_qtiles; b0 += 64) {
+      const int blk = b0 + lane;
+      int f = 0;
+      if (blk < 2 * n_qtiles) {
+        f = (bits[2 * i * words + blk / 32] >> (blk % 32)) & 1;
+        f |= ((bits[(2 * i + 1) * words + blk / 32] >> (blk % 32)) & 1) << 1;
+      }
+      const uint64_t on = __ballot(f != 0);
+      if (f) list[n + __builtin_popcountll(on & ((1ull << lane) - 1))] = (blk << 2) | f;
+      n += __builtin_popcountll(on);
+    }
+    if (lane == 0) out_counts[slot] = n;
+  }
+}
+
+}  // namespace
+}  // namespace moddit
+
+extern "C" int64_t moddit_attention_bwd_workspace_bytes(int batch, int heads, int q_len, int kv_len, int head_dim,
+                                                        int dtype, int grid_origin) {
+  using namespace moddit;
+  if (batch <= 0 || heads <= 0 || q_len < 0 || kv_len < 0 || grid_origin > 0 || grid_origin <= -kBN) return 0;
+  return bwd_workspace_floats(batch, heads, q_len, kv_len, dtype, grid_origin) * 4;
+}
+
+extern "C" int moddit_flash_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse,
+                                const void* grad_o, const float* grad_lse, void* dq, void* dk, void* dv, int batch,
+                                int heads, int q_len, int kv_len, int head_dim, const int64_t q_strides[3],
+                                const int64_t k_strides[3], const int64_t v_strides[3], const int64_t o_strides[3],
+                                const int64_t go_strides[3], const int64_t dq_strides[3], const int64_t dk_strides[3],
+                                const int64_t dv_strides[3], float softmax_scale, int dtype, void* workspace,
+                                int64_t workspace_bytes, moddit_stream_t stream) {
+  const moddit::BwdArgs a{q, k, v, o, grad_o, lse, grad_lse, dq, dk, dv, batch, heads, q_len, kv_len, head_dim,
+                          q_strides, k_strides, v_strides, o_strides, go_strides, dq_strides, dk_strides, dv_strides,
+                          softmax_scale, dtype, nullptr, nullptr, 0, 0, nullptr, nullptr, 0, 0, 0, workspace,
+                          workspace_bytes};
+  return moddit::bwd_entry(a, stream);
+}
+
+extern "C" int moddit_block_sparse_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse,
+                                       const void* grad_o, const float* grad_lse, void* dq, void* dk, void* dv,
+                                       int batch, int heads, int q_len, int kv_len, int head_dim,
+                                       const int64_t q_strides[3], const int64_t k_strides[3],
+                                       const int64_t v_strides[3], const int64_t o_strides[3],
+                                       const int64_t go_strides[3], const int64_t dq_strides[3],
+                                       const int64_t dk_strides[3], const int64_t dv_strides[3], float softmax_scale,
+                                       int dtype, const int32_t* counts, const int32_t* entries, int n_qtiles, int cap,
+                                       const int32_t* key_counts, const int32_t* key_entries, int n_ktiles,
+                                       int key_cap, int grid_origin, void* workspace, int64_t workspace_bytes,
+                                       moddit_stream_t stream) {
+  if (counts == nullptr) {
+    moddit::set_error("block_sparse_bwd: counts must not be NULL");
+    return MODDIT_EINVAL;
+  }
+  const moddit::BwdArgs a{q, k, v, o, grad_o, lse, grad_lse, dq, dk, dv, batch, heads, q_len, kv_len, head_dim,
+                          q_strides, k_strides, v_strides, o_strides, go_strides, dq_strides, dk_strides, dv_strides,
+                          softmax_scale, dtype, counts, entries, n_qtiles, cap, key_counts, key_entries, n_ktiles,
+                          key_cap, grid_origin, workspace, workspace_bytes};
+  return moddit::bwd_entry(a, stream);
+}
+
+extern "C" int moddit_transpose_tiles(const int32_t* counts, const int32_t* entries, int heads, int n_qtiles, int cap,
+                                      int32_t* key_counts, int32_t* key_entries, int n_ktiles, int key_cap,
+                                      moddit_stream_t stream) {
+  using namespace moddit;
+  clear_error();
+  MODDIT_CHECK_ARG(heads >= 0 && heads <= 65535 && n_qtiles >= 0 && n_ktiles >= 0 && cap >= 0, "transpose_tiles: bad size");
+  if (2 * static_cast<int64_t>(n_qtiles) > kMaxBlocks) {
+    set_error("transpose_tiles: n_qtiles=%d exceeds %d", n_qtiles, kMaxBlocks / 2);
+    return MODDIT_EUNSUPPORTED;
+  }
+  MODDIT_CHECK_ARG(key_cap == 2 * n_qtiles, "transpose_tiles: key_cap=%d must be 2 * n_qtiles=%d", key_cap, 2 * n_qtiles);
+  if (heads == 0 || n_ktiles == 0) return MODDIT_OK;
+  MODDIT_CHECK_ARG(key_counts && (n_qtiles == 0 || (counts && key_entries && (entries || cap == 0))), "transpose_tiles: null pointer");
+  const int words = (2 * n_qtiles + 31) / 32;
+  hipLaunchKernelGGL(transpose_tiles_kernel, dim3((n_ktiles + kPairs - 1) / kPairs, heads), dim3(kThreads),
+                     2 * kPairs * words * 4, as_stream(stream), counts, entries, n_qtiles, cap, n_ktiles, words,
+                     key_counts, key_entries);
+  MODDIT_CHECK_LAUNCH("transpose_tiles");
+  return MODDIT_OK;
+}

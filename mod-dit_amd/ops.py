@@ -14,7 +14,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._lib import check, strides3
+from ._lib import check, strides2, strides3
 
 _DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
 
@@ -33,11 +33,20 @@ def _require_gpu(*tensors: torch.Tensor, what: str) -> None:
             raise ValueError(f"{what}: tensors must live on a GPU (got {t.device})")
 
 
+def _kernel_strides(t: torch.Tensor) -> bool:
+    """Whether the kernels can address (B,H,S,D) t: unit dim stride, 16-byte aligned rows."""
+    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in t.stride()[:3])
+
+
 def _attn_view(t: torch.Tensor) -> torch.Tensor:
     """(B,H,S,D) with unit dim stride, 16-byte aligned; copies only if needed."""
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:3]):
-        t = t.contiguous()
-    return t
+    return t if _kernel_strides(t) else t.contiguous()
+
+
+def _empty_as(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised tensor of t's shape, dtype and order of dimensions, as the kernels write."""
+    out = torch.empty_like(t)
+    return out if _kernel_strides(out) else torch.empty(t.shape, device=t.device, dtype=t.dtype)
 
 
 def _attn_dtype(t: torch.Tensor) -> int:
@@ -184,6 +193,271 @@ def flash_fwd_map(q, k, v, *, softmax_scale, log_threshold, video_offset, video_
         float(log_threshold), int(video_offset), int(video_blocks), int(block_size), dt,
         _stream(q)), "moddit_flash_fwd_map")
     return out, lse, smap
+
+
+# --------------------------------------------------------------------------------------
+# gradients of attention
+# --------------------------------------------------------------------------------------
+@dataclass
+class KeyTileList:
+    """A TileList's pairs by key tile, for the gradients of keys and values: per (head, 128-key
+    tile) ascending lists of the 64-row query blocks that attend to it.
+
+    entries[h, t, i] = (query_block << 2) | key_bits for i < counts[h, t]; bit 0 stands for keys
+    0..63 of the key tile, bit 1 for keys 64..127. The grid is the TileList's.
+    """
+
+    counts: torch.Tensor   # (H, n_ktiles) int32
+    entries: torch.Tensor  # (H, n_ktiles, cap) int32
+    origin: int = 0
+
+    @property
+    def n_ktiles(self) -> int:
+        return self.counts.shape[1]
+
+    @property
+    def cap(self) -> int:
+        return self.entries.shape[2]
+
+
+_MAX_QTILES = 6144  # query tiles whose transposed bits fit a workgroup's LDS
+
+
+def transpose_tiles(tiles: TileList, kv_len: int) -> KeyTileList:
+    """The KeyTileList of `tiles` for kv_len keys. A program that trains under one mask for several
+    calls keeps it and hands it to `block_sparse_bwd`."""
+    _require_gpu(tiles.counts, tiles.entries, what="transpose_tiles")
+    H, nq = tiles.counts.shape
+    if kv_len < 0:
+        raise ValueError(f"kv_len must not be negative, got {kv_len}")
+    if nq > _MAX_QTILES:
+        raise ValueError(f"transpose_tiles takes at most {_MAX_QTILES} query tiles, got {nq}")
+    _check_tiles(tiles, "transpose_tiles")
+    device = tiles.counts.device
+    nk = (int(kv_len) - tiles.origin + 127) // 128
+    out = KeyTileList(torch.empty((H, nk), device=device, dtype=torch.int32),
+                      torch.empty((H, nk, 2 * nq), device=device, dtype=torch.int32), int(tiles.origin))
+    with torch.cuda.device(device):
+        check(_lib.load().moddit_transpose_tiles(
+            tiles.counts.data_ptr(), tiles.entries.data_ptr(), H, nq, tiles.cap, out.counts.data_ptr(),
+            out.entries.data_ptr(), nk, out.cap, _stream(tiles.counts)), "moddit_transpose_tiles")
+    return out
+
+
+def _check_tiles(tiles, what):
+    """Lists as the kernels index them: int32, contiguous, of one size."""
+    c, e = tiles.counts, tiles.entries
+    if c.ndim != 2 or e.ndim != 3 or e.shape[:2] != c.shape or c.dtype != torch.int32 or \
+            e.dtype != torch.int32 or not c.is_contiguous() or not e.is_contiguous() or c.device != e.device:
+        raise ValueError(f"{what}: tile lists must be contiguous int32 counts (H, n) and entries (H, n, cap) "
+                         "on one device")
+
+
+def _attention_bwd(what, q, k, v, out, lse, grad_out, scale, grad_lse, tiles, key_tiles):
+    lists = [t for l in (tiles, key_tiles) if l is not None for t in (l.counts, l.entries)]
+    device = _same_device(what, q, k, v, out, lse, grad_out, grad_lse, *lists)
+    if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
+        raise ValueError("query, key and value must have shape [B, H, S, D]")
+    if k.shape != v.shape or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"incompatible shapes q={tuple(q.shape)} k={tuple(k.shape)} v={tuple(v.shape)}")
+    if out.shape != q.shape or grad_out.shape != q.shape:
+        raise ValueError(f"{what}: out and grad_out must have query's shape {tuple(q.shape)}, got "
+                         f"{tuple(out.shape)} and {tuple(grad_out.shape)}")
+    if any(t.dtype != q.dtype for t in (k, v, out, grad_out)):
+        raise ValueError(f"{what}: query, key, value, out and grad_out must have the same dtype")
+    dt = _attn_dtype(q)
+    B, H, Sq, D = q.shape
+    Skv = k.shape[2]
+    if D not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, got {D}")
+    for t, name in ((lse, "lse"), (grad_lse, "grad_lse")):
+        if t is not None and (t.shape != (B, H, Sq) or t.dtype != torch.float32):
+            raise ValueError(f"{what}: {name} must be float32 of shape {(B, H, Sq)}, got {t.dtype} "
+                             f"{tuple(t.shape)}")
+    if B * H > 65535:
+        raise ValueError(f"{what}: batch * heads exceeds 65535")
+    origin = 0
+    if tiles is not None:
+        _check_tiles(tiles, what)
+        origin = int(tiles.origin)
+        if tiles.counts.shape[0] != H:
+            raise ValueError(f"tile lists cover {tiles.counts.shape[0]} heads, attention has {H}")
+        if key_tiles is None:
+            key_tiles = transpose_tiles(tiles, Skv)
+        _check_tiles(key_tiles, what)
+        if key_tiles.counts.shape[0] != H or key_tiles.origin != origin or key_tiles.cap != 2 * tiles.n_qtiles:
+            raise ValueError(f"{what}: key_tiles are not the transposed lists of tiles")
+    q, k, v, out, grad_out = (_attn_view(t) for t in (q, k, v, out, grad_out))
+    lse, grad_lse = (None if t is None else t.contiguous() for t in (lse, grad_lse))
+    dq, dk, dv = _empty_as(q), _empty_as(k), _empty_as(v)
+    lib = _lib.load()
+    nbytes = _split_bytes("moddit_attention_bwd_workspace_bytes", B, H, Sq, Skv, D, dt, origin)
+    ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
+    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), grad_out.data_ptr(),
+            _ptr(grad_lse), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, H, Sq, Skv, D,
+            *(strides3(*t.stride()[:3]) for t in (q, k, v, out, grad_out, dq, dk, dv)),
+            float(D ** -0.5 if scale is None else scale), dt)
+    with torch.cuda.device(device):
+        if tiles is None:
+            check(lib.moddit_flash_bwd(*args, ws.data_ptr(), nbytes, _stream(q)), "moddit_flash_bwd")
+        else:
+            check(lib.moddit_block_sparse_bwd(
+                *args, *(x for l, n in ((tiles, tiles.n_qtiles), (key_tiles, key_tiles.n_ktiles))
+                         for x in (l.counts.data_ptr(), l.entries.data_ptr(), n, l.cap)),
+                origin, ws.data_ptr(), nbytes, _stream(q)), "moddit_block_sparse_bwd")
+    return dq, dk, dv
+
+
+def flash_bwd(q, k, v, out, lse, grad_out, softmax_scale=None, grad_lse=None):
+    """Gradients (dq, dk, dv) of `flash_fwd` at q, k, v, for the gradient of its output and, where
+    it is given, of its LSE (B,H,Sq) fp32. out and lse are the forward's. Results repeat bit for bit."""
+    return _attention_bwd("flash_bwd", q, k, v, out, lse, grad_out, softmax_scale, grad_lse, None, None)
+
+
+def block_sparse_bwd(q, k, v, out, lse, grad_out, tiles: TileList, softmax_scale=None, grad_lse=None,
+                     key_tiles: KeyTileList | None = None):
+    """Gradients (dq, dk, dv) of `block_sparse_fwd` under the same tiles. key_tiles:
+    `transpose_tiles(tiles, kv_len)` where the caller keeps it; built here otherwise."""
+    return _attention_bwd("block_sparse_bwd", q, k, v, out, lse, grad_out, softmax_scale, grad_lse, tiles,
+                          key_tiles)
+
+
+# --------------------------------------------------------------------------------------
+# norm and rotation of queries and keys
+# --------------------------------------------------------------------------------------
+_NORMS = {"none": _lib.NORM_NONE, "rms": _lib.NORM_RMS, "layer": _lib.NORM_LAYER}
+_WEIGHT_DTYPES = {**_DTYPES, torch.float32: _lib.FP32}
+_MAX_NORM_ROW = 8192
+
+
+def _same_device(what, *tensors):
+    """All tensors (None aside) on the first one's GPU, which is returned."""
+    got = [t for t in tensors if t is not None]
+    _require_gpu(*got, what=what)
+    if any(t.device != got[0].device for t in got):
+        raise ValueError(f"{what}: tensors must live on the same GPU")
+    return got[0].device
+
+
+def _qk_norm_args(what, q, k, norm, across_heads, eps, weights, biases, cos, sin, rope_offset):
+    """Checks of qk_norm_rope's arguments; (batch, heads, q_len, k_len, dim), the C call's tail of
+    norm, weights and tables, and what that tail points into."""
+    if q.ndim != 4 or k.ndim != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"{what}: q and k must have shapes [B, H, S, D] that differ in S at most, got "
+                         f"{tuple(q.shape)} and {tuple(k.shape)}")
+    if q.dtype != k.dtype:
+        raise ValueError(f"{what}: q and k must have the same dtype")
+    _attn_dtype(q)
+    B, H, Sq, D = q.shape
+    if D not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, got {D}")
+    if norm not in _NORMS:
+        raise ValueError(f"norm must be one of {sorted(_NORMS)}, got {norm!r}")
+    affine = [t for t in (*weights, *biases) if t is not None]
+    if norm == "none" and (affine or across_heads):
+        raise ValueError(f"{what}: weights, biases and across_heads need a norm")
+    if across_heads and H * D > _MAX_NORM_ROW:
+        raise ValueError(f"{what}: a norm over all heads takes heads * head_dim <= {_MAX_NORM_ROW}, "
+                         f"got {H * D}")
+    if not 0.0 <= eps < math.inf:
+        raise ValueError(f"{what}: eps must be finite and not negative, got {eps}")
+    n = H * D if across_heads else D
+    for t in affine:
+        if t.shape != (n,):
+            raise ValueError(f"{what}: weights and biases must have shape ({n},), got {tuple(t.shape)}")
+        if t.dtype not in _WEIGHT_DTYPES or t.dtype != affine[0].dtype:
+            raise TypeError(f"{what}: weights and biases must share one of float16, bfloat16 and float32")
+    if (cos is None) != (sin is None):
+        raise ValueError(f"{what}: cos and sin come together")
+    tab, rows, width = (0, 0), 0, 0
+    if cos is not None:
+        if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+            raise TypeError(f"{what}: cos and sin must be float32")
+        if cos.shape != sin.shape or cos.ndim not in (2, 3) or cos.shape[-1] not in (D, D // 2) or \
+                (cos.ndim == 3 and cos.shape[0] != B):
+            raise ValueError(f"{what}: cos and sin must have shape [n, {D}], [n, {D // 2}] or the same with "
+                             f"the batch in front, got {tuple(cos.shape)} and {tuple(sin.shape)}")
+        if cos.stride() != sin.stride() or cos.stride(-1) != 1:
+            cos, sin = cos.contiguous(), sin.contiguous()
+        rows, width = cos.shape[-2:]
+        if not 0 <= rope_offset <= min(Sq, k.shape[2]) - rows:
+            raise ValueError(f"{what}: rotated tokens [{rope_offset}, {rope_offset + rows}) exceed the "
+                             f"{min(Sq, k.shape[2])} tokens of the shorter tensor")
+        tab = (cos.stride(0) if cos.ndim == 3 else 0, cos.stride(-2))
+    weights, biases = ([None if t is None else t.contiguous() for t in ts] for ts in (weights, biases))
+    head = (_NORMS[norm], int(bool(across_heads)), float(eps))
+    affine_dtype = _WEIGHT_DTYPES[affine[0].dtype] if affine else _lib.FP32
+    tables = (_ptr(cos) if rows else None, _ptr(sin) if rows else None, strides2(*tab), int(width),
+              int(rope_offset) if rows else 0, int(rows))
+    return (B, H, Sq, k.shape[2], D), head, (weights, biases, affine_dtype), tables, (cos, sin)
+
+
+def qk_norm_rope(q, k, *, norm="rms", across_heads=False, eps=1e-6, q_weight=None, k_weight=None,
+                 q_bias=None, k_bias=None, cos=None, sin=None, rope_offset=0, interleaved=True, out=None):
+    """Norm of queries and keys and the rotation of their positions in one pass; returns (q', k').
+
+    q, k (B,H,S,D) bf16/fp16 (S may differ). norm: 'rms', 'layer' or 'none', over each head's D, or
+    over all heads' H*D of a token with `across_heads`; weights and biases have as many values and
+    may be left out. cos, sin (n, D) or (n, D/2) fp32, or with the batch in front, turn the tokens
+    [rope_offset, rope_offset + n) of both: pairs (2i, 2i+1) with `interleaved`, else (i, i + D/2). In
+    a table of D values a pair's cos is read at its first element and its sin at its second. out:
+    a pair of tensors to write, which may be q and k themselves."""
+    what = "qk_norm_rope"
+    device = _same_device(what, q, k, q_weight, k_weight, q_bias, k_bias, cos, sin)
+    sizes, head, (w, b, w_dt), tables, keep = _qk_norm_args(
+        what, q, k, norm, across_heads, eps, (q_weight, k_weight), (q_bias, k_bias), cos, sin, rope_offset)
+    if out is None:
+        out = tuple(_empty_as(t) for t in (q, k))
+    else:
+        q_out, k_out = out = tuple(out)
+        for t, like in ((q_out, q), (k_out, k)):
+            if t.shape != like.shape or t.dtype != like.dtype or t.device != device:
+                raise ValueError(f"{what}: out must be of the shapes, dtype and device of q and k")
+            if not _kernel_strides(t):
+                raise ValueError(f"{what}: out needs a unit dim stride, 16-byte alignment and strides of "
+                                 "multiples of 8 elements")
+    q, k = _attn_view(q), _attn_view(k)
+    with torch.cuda.device(device):
+        check(_lib.load().moddit_qk_norm_rope(
+            q.data_ptr(), k.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), *sizes,
+            *(strides3(*t.stride()[:3]) for t in (q, k, *out)), _attn_dtype(q), *head,
+            _ptr(w[0]), _ptr(w[1]), _ptr(b[0]), _ptr(b[1]), w_dt, *tables, int(bool(interleaved)),
+            _stream(q)), "moddit_qk_norm_rope")
+    return out
+
+
+def qk_norm_rope_bwd(q, k, grad_q, grad_k, *, norm="rms", across_heads=False, eps=1e-6, q_weight=None,
+                     k_weight=None, q_bias=None, k_bias=None, cos=None, sin=None, rope_offset=0,
+                     interleaved=True):
+    """Gradients of `qk_norm_rope` at q, k for the gradients of its outputs.
+
+    Returns (dq, dk, dq_weight, dk_weight, dq_bias, dk_bias): dq and dk in q's dtype, the others
+    fp32, None for a weight or bias that is None."""
+    what = "qk_norm_rope_bwd"
+    device = _same_device(what, q, k, grad_q, grad_k, q_weight, k_weight, q_bias, k_bias, cos, sin)
+    sizes, head, (w, b, w_dt), tables, keep = _qk_norm_args(
+        what, q, k, norm, across_heads, eps, (q_weight, k_weight), (q_bias, k_bias), cos, sin, rope_offset)
+    for t, like in ((grad_q, q), (grad_k, k)):
+        if t.shape != like.shape or t.dtype != like.dtype:
+            raise ValueError(f"{what}: grad_q and grad_k must have the shapes and dtype of q and k")
+    q, k, grad_q, grad_k = (_attn_view(t) for t in (q, k, grad_q, grad_k))
+    dq, dk = _empty_as(q), _empty_as(k)
+    empty = sizes[0] * sizes[1] * max(sizes[2], sizes[3]) == 0
+    sums = [None if t is None else (torch.zeros if empty else torch.empty)(t.shape, device=device, dtype=torch.float32)
+            for t in (*w, *b)]
+    lib = _lib.load()
+    ws, floats = None, 0
+    if any(t is not None for t in sums) and not empty:
+        floats = lib.moddit_qk_norm_rope_bwd_workspace_floats(*sizes, head[1])
+        ws = torch.empty(floats, device=device, dtype=torch.float32)
+    with torch.cuda.device(device):
+        check(lib.moddit_qk_norm_rope_bwd(
+            q.data_ptr(), k.data_ptr(), grad_q.data_ptr(), grad_k.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+            *(_ptr(t) for t in sums), *sizes,
+            *(strides3(*t.stride()[:3]) for t in (q, k, grad_q, grad_k, dq, dk)), _attn_dtype(q), *head,
+            _ptr(w[0]), _ptr(w[1]), w_dt, *tables, int(bool(interleaved)), _ptr(ws), floats, _stream(q)),
+            "moddit_qk_norm_rope_bwd")
+    return (dq, dk, *sums)
 
 
 # --------------------------------------------------------------------------------------

@@ -46,14 +46,20 @@ __device__ __forceinline__ s16x4 lds_read_tr16(const unsigned char* a) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a));
 }
 
-template <int D>
+// At D = 128 the dK/dV pass has no registers for V beside its sums (128) and K (32): V stays in
+// LDS, and stages are half a tile so that two workgroups fit a CU.
+template <int D, bool kKeys>
 struct BwdLds {
+  static constexpr bool kOwn2InLds = kKeys && D == 128;
+  static constexpr int kRows = kOwn2InLds ? 32 : kBN;  // streamed rows of a stage
+  static constexpr int kSteps = kBN / kRows;           // stages of a tile
   static constexpr int kRowBytes = D * 2;
-  static constexpr int kTileBytes = kBN * kRowBytes;
+  static constexpr int kTileBytes = kRows * kRowBytes;  // one tensor's part of a stage
   static constexpr int kRowsPerWindow = 1024 / kRowBytes;
   static constexpr int kWinPerWave = kTileBytes / 1024 / 4;
-  static constexpr int kStage = 2 * kTileBytes + kStatsBytes;
-  static constexpr int kTotal = 2 * kStage;
+  static constexpr int kStage = 2 * kTileBytes + (kKeys ? kStatsBytes : 0);
+  static constexpr int kOwn2Bytes = kOwn2InLds ? kBM * kRowBytes : 0;
+  static constexpr int kTotal = 2 * kStage + kOwn2Bytes;
 };
 
 // XOR on the 16-byte chunks of LDS row r. Both reads of a tile are free of bank conflicts: the
@@ -222,8 +228,8 @@ __device__ __forceinline__ int ds_exponent(const float* maxima, int n, float (*r
 }
 
 template <int D, typename E, bool kKeys, bool kSparse>
-__global__ __launch_bounds__(kThreads, D == 128 && kKeys ? 1 : 2) void attention_bwd_kernel(BwdParams p) {
-  using L = BwdLds<D>;
+__global__ __launch_bounds__(kThreads, 2) void attention_bwd_kernel(BwdParams p) {
+  using L = BwdLds<D, kKeys>;
   using V8 = typename E::vec8;
   constexpr int kKC = D / 32;  // MFMA k-steps over d
   constexpr int kDB = D / 16;  // 16-row blocks of the transposed sums
@@ -265,7 +271,7 @@ __global__ __launch_bounds__(kThreads, D == 128 && kKeys ? 1 : 2) void attention
 
   // ---- owned rows (B operands): lane holds row 16qq + c16, dims 32c + 8g.. ----
   const int row0 = p.origin + ot * kBM + wave * 32 + c16;
-  V8 own1[2][kKC], own2[2][kKC];
+  V8 own1[2][kKC], own2[2][L::kOwn2InLds ? 1 : kKC];
 #pragma unroll
   for (int qq = 0; qq < 2; ++qq) {
     const int row = row0 + 16 * qq;
@@ -275,7 +281,7 @@ __global__ __launch_bounds__(kThreads, D == 128 && kKeys ? 1 : 2) void attention
 #pragma unroll
     for (int i = 0; i < kKC; ++i) {
       own1[qq][i] = as_vec8<V8>(a[4 * i + g]);
-      own2[qq][i] = as_vec8<V8>(c[4 * i + g]);
+      if constexpr (!L::kOwn2InLds) own2[qq][i] = as_vec8<V8>(c[4 * i + g]);
     }
   }
   const float* stats = p.stats + static_cast<int64_t>(bh) * p.stat_blocks * 128;
@@ -306,18 +312,32 @@ __global__ __launch_bounds__(kThreads, D == 128 && kKeys ? 1 : 2) void attention
     src1[i] = static_cast<uint32_t>(((p.origin + r) * static_cast<int>(p.str1.ss) + ch * 8) * 2);
     src2[i] = static_cast<uint32_t>(((p.origin + r) * static_cast<int>(p.str2.ss) + ch * 8) * 2);
   }
-  const uint32_t step1 = static_cast<uint32_t>(kBN * p.str1.ss * 2);
-  const uint32_t step2 = static_cast<uint32_t>(kBN * p.str2.ss * 2);
-  auto dma = [&](int st, int stage) {
+  const uint32_t step1 = static_cast<uint32_t>(L::kRows * p.str1.ss * 2);
+  const uint32_t step2 = static_cast<uint32_t>(L::kRows * p.str2.ss * 2);
+  auto dma = [&](int st, int part, int stage) {
     const uint32_t dst = lds0 + stage * L::kStage;
+    const uint32_t at = st * L::kSteps + part;
 #pragma unroll
     for (int i = 0; i < L::kWinPerWave; ++i)
-      lds_dma16(rsrc1, dst + (wave * L::kWinPerWave + i) * 1024, src1[i] + st * step1, 0);
+      lds_dma16(rsrc1, dst + (wave * L::kWinPerWave + i) * 1024, src1[i] + at * step1, 0);
 #pragma unroll
     for (int i = 0; i < L::kWinPerWave; ++i)
-      lds_dma16(rsrc2, dst + L::kTileBytes + (wave * L::kWinPerWave + i) * 1024, src2[i] + st * step2, 0);
+      lds_dma16(rsrc2, dst + L::kTileBytes + (wave * L::kWinPerWave + i) * 1024, src2[i] + at * step2, 0);
     if (kKeys && wave == 0) lds_dma16(rsrc_st, dst + 2 * L::kTileBytes, lane * 16 + st * 512, 0);
   };
+  const unsigned char* const own2_lds = smem + 2 * L::kStage + wave * 32 * L::kRowBytes;
+  if constexpr (L::kOwn2InLds) {
+    const int64_t span = (static_cast<int64_t>(p.own_len) - 1) * p.own2.ss * 2 + L::kRowBytes;
+    const u32x4 rsrc = raw_rsrc(p.own2.p + b * p.own2.sb + h * p.own2.sh, static_cast<uint32_t>(span));
+#pragma unroll
+    for (int i = 0; i < L::kOwn2Bytes / 1024 / 4; ++i) {
+      const int w = wave * (L::kOwn2Bytes / 1024 / 4) + i;
+      const int r = w * L::kRowsPerWindow + (lane * 16) / L::kRowBytes;
+      const int ch = (((lane * 16) % L::kRowBytes) / 16) ^ swz<D>(r);
+      const uint32_t off = static_cast<uint32_t>(((p.origin + ot * kBM + r) * static_cast<int>(p.own2.ss) + ch * 8) * 2);
+      lds_dma16(rsrc, lds0 + 2 * L::kStage + w * 1024, off, 0);
+    }
+  }
 
   // ---- LDS operand addressing ----
   uint32_t row_rd[kKC];  // A operand of S and dP: row 16sb + c16, logical chunk 4c + g
@@ -355,7 +375,10 @@ __global__ __launch_bounds__(kThreads, D == 128 && kKeys ? 1 : 2) void attention
   };
 
   // 32 streamed rows (half t of the tile) against the wave's 32 owned ones
-  auto half_tile = [&](const unsigned char* t1, const unsigned char* t2, const float* stt, int t, int st) {
+  auto half_tile = [&](const unsigned char* stage, int t, int st) {
+    const unsigned char* t1 = stage + (L::kSteps == 1 ? t * 32 * L::kRowBytes : 0);
+    const unsigned char* t2 = t1 + L::kTileBytes;
+    const float* stt = reinterpret_cast<const float*>(stage + 2 * L::kTileBytes);
     f32x4 s[2][2], dp[2][2], nl[2];
 #pragma unroll
     for (int sb = 0; sb < 2; ++sb) {
@@ -374,7 +397,7 @@ __global__ __launch_bounds__(kThreads, D == 128 && kKeys ? 1 : 2) void attention
     for (int c = 0; c < kKC; ++c)
 #pragma unroll
       for (int sb = 0; sb < 2; ++sb) {
-        const V8 a = *reinterpret_cast<const V8*>(t1 + row_rd[c] + (32 * t + 16 * sb) * L::kRowBytes);
+        const V8 a = *reinterpret_cast<const V8*>(t1 + row_rd[c] + 16 * sb * L::kRowBytes);
         s[sb][0] = E::mma16(a, own1[0][c], s[sb][0]);
         s[sb][1] = E::mma16(a, own1[1][c], s[sb][1]);
       }
@@ -382,9 +405,15 @@ __global__ __launch_bounds__(kThreads, D == 128 && kKeys ? 1 : 2) void attention
     for (int c = 0; c < kKC; ++c)
 #pragma unroll
       for (int sb = 0; sb < 2; ++sb) {
-        const V8 a = *reinterpret_cast<const V8*>(t2 + row_rd[c] + (32 * t + 16 * sb) * L::kRowBytes);
-        dp[sb][0] = E::mma16(a, own2[0][c], dp[sb][0]);
-        dp[sb][1] = E::mma16(a, own2[1][c], dp[sb][1]);
+        const V8 a = *reinterpret_cast<const V8*>(t2 + row_rd[c] + 16 * sb * L::kRowBytes);
+        if constexpr (L::kOwn2InLds) {
+#pragma unroll
+          for (int qq = 0; qq < 2; ++qq)
+            dp[sb][qq] = E::mma16(a, *reinterpret_cast<const V8*>(own2_lds + row_rd[c] + 16 * qq * L::kRowBytes), dp[sb][qq]);
+        } else {
+          dp[sb][0] = E::mma16(a, own2[0][c], dp[sb][0]);
+          dp[sb][1] = E::mma16(a, own2[1][c], dp[sb][1]);
+        }
       }
     if constexpr (!kKeys) {
       const int key0 = p.origin + st * kBN;
@@ -417,11 +446,11 @@ __global__ __launch_bounds__(kThreads, D == 128 && kKeys ? 1 : 2) void attention
         }
 #pragma unroll
     for (int db = 0; db < kDB; ++db) {
-      const V8 a = tr_operand(t1 + tr_rd[db] + t * 32 * L::kRowBytes);
+      const V8 a = tr_operand(t1 + tr_rd[db]);
       acc1[db][0] = E::mma16(a, db_[0], acc1[db][0]);
       acc1[db][1] = E::mma16(a, db_[1], acc1[db][1]);
       if constexpr (kKeys) {
-        const V8 c = tr_operand(t2 + tr_rd[db] + t * 32 * L::kRowBytes);
+        const V8 c = tr_operand(t2 + tr_rd[db]);
         acc2[db][0] = E::mma16(c, pb[0], acc2[db][0]);
         acc2[db][1] = E::mma16(c, pb[1], acc2[db][1]);
       }
@@ -431,21 +460,23 @@ __global__ __launch_bounds__(kThreads, D == 128 && kKeys ? 1 : 2) void attention
   int st = 0, flags = 0;
   if (n_iter > 0) {
     decode(entry(0), st, flags);
-    dma(st, 0);
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
+    dma(st, 0, 0);
   }
-  for (int j = 0; j < n_iter; ++j) {
-    int st1 = 0, flags1 = 0;
-    if (j + 1 < n_iter) {
-      decode(entry(j + 1), st1, flags1);
-      dma(st1, (j + 1) & 1);
+  __builtin_amdgcn_s_waitcnt(0);  // V's DMA too, which must not outlive the workgroup
+  __syncthreads();
+  const int n_steps = n_iter * L::kSteps;
+  for (int j = 0; j < n_steps; ++j) {
+    const int part = j % L::kSteps;
+    int st1 = st, flags1 = flags;
+    if (j + 1 < n_steps) {
+      if (part == L::kSteps - 1) decode(entry((j + 1) / L::kSteps), st1, flags1);
+      dma(st1, (j + 1) % L::kSteps, (j + 1) & 1);
     }
     __builtin_amdgcn_sched_barrier(0);
-    const unsigned char* t1 = smem + (j & 1) * L::kStage;
+    const unsigned char* stage = smem + (j & 1) * L::kStage;
     if (flags & wbit) {
-      half_tile(t1, t1 + L::kTileBytes, reinterpret_cast<const float*>(t1 + 2 * L::kTileBytes), 0, st);
-      half_tile(t1, t1 + L::kTileBytes, reinterpret_cast<const float*>(t1 + 2 * L::kTileBytes), 1, st);
+      half_tile(stage, part, st);
+      if (L::kSteps == 1) half_tile(stage, 1, st);
     }
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
@@ -482,7 +513,7 @@ __global__ __launch_bounds__(kThreads, D == 128 && kKeys ? 1 : 2) void attention
 
 template <int D, typename E, bool kKeys, bool kSparse>
 int launch_pass(const BwdParams& p, int batch, hipStream_t st) {
-  constexpr int kLds = BwdLds<D>::kTotal;
+  constexpr int kLds = BwdLds<D, kKeys>::kTotal;
   auto kernel = attention_bwd_kernel<D, E, kKeys, kSparse>;
   static LaunchSetup once;
   if (set_dynamic_lds_once(once, reinterpret_cast<const void*>(kernel), kLds) != hipSuccess) {

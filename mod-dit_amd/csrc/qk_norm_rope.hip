@@ -44,6 +44,7 @@ struct RopeParams {
   int heads;
   int dim;
   int w_type;  // moddit_dtype of w and b
+  int has_bias;  // a bias is added, or its gradient asked for
   float eps;
   const float* cos;
   const float* sin;
@@ -296,11 +297,98 @@ __global__ __launch_bounds__(kThreads) void norm_rope_heads_kernel(RopeParams p)
   }
 }
 
-// ---- norm over all heads of a token ----
-// One workgroup per token and tensor at a time; a thread holds kChunks groups of 8 elements, and
-// their weights across tokens.
-template <int kChunks, typename E, int kNorm, bool kInter, bool kBwd>
-__global__ __launch_bounds__(kThreads) void norm_rope_token_kernel(RopeParams p) {
+// ---- norm over all heads of a token, forward ----
+// One wave per token and tensor at a time, all its loads (kChunks of 16 bytes a lane) in flight
+// together and no barrier; the weights wait in LDS as fp32, in two halves of 16 bytes a group of
+// 8 elements so that a wave's reads are contiguous.
+template <int kChunks, typename E, int kNorm, bool kInter, bool kBias>
+__global__ __launch_bounds__(kThreads) void norm_rope_wave_kernel(RopeParams p) {
+  extern __shared__ float affine[];  // [w, bias][2][n_chunks][4]
+  const RopeTensor q = p.t[blockIdx.y];
+  const int lanes = p.dim / 8;
+  const int n_chunks = p.heads * lanes;
+  const float inv_n = 1.f / (p.heads * p.dim);
+  for (int i = threadIdx.x; i < n_chunks * 8; i += kThreads) {
+    const int ch = i >> 3, e = i & 7;
+    const int src = ch / lanes * p.dim + col_of<kInter>(ch % lanes, e, p.dim);
+    const int dst = ((e >> 2) * n_chunks + ch) * 4 + (e & 3);
+    affine[dst] = affine_at(q.w, p.w_type, src, 1.f);
+    if (kBias) affine[8 * n_chunks + dst] = affine_at(q.b, p.w_type, src, 0.f);
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 63;
+  const int l = lane % lanes;
+  const int h0 = lane / lanes, h_step = 64 / lanes;
+  auto wave_sum = [](float x) {
+    x = row_sum<16>(x);
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+  };
+
+  const int64_t items = static_cast<int64_t>(p.batch) * q.len;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kWaves;
+  for (int64_t item = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6); item < items; item += step) {
+    const int b = static_cast<int>(item / q.len);
+    const int token = static_cast<int>(item % q.len);
+    const uint16_t* src = q.x + b * q.x_sb + token * q.x_ss + h0 * q.x_sh;
+    uint16_t* dst = q.y + b * q.y_sb + token * q.y_ss + h0 * q.y_sh;
+    u32x4 raw[kChunks];
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j)
+      raw[j] = lane + 64 * j < n_chunks ? load_row<kInter>(src + j * h_step * q.x_sh, l, p.dim) : u32x4{0, 0, 0, 0};
+    float c[4], s[4];
+    load_angles<kInter>(p, b, token, l, c, s);
+    float mu = 0.f, sq = 0.f;
+    if (kNorm == kLayer) {
+#pragma unroll
+      for (int j = 0; j < kChunks; ++j) {
+        float x[8];
+        unpack<E>(raw[j], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mu += x[e];
+      }
+      mu = wave_sum(mu) * inv_n;
+    }
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) {
+      float x[8], part = 0.f;
+      unpack<E>(raw[j], x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) part += (x[e] - mu) * (x[e] - mu);
+      if (kNorm != kLayer || lane + 64 * j < n_chunks) sq += part;
+    }
+    const float r = rsqrtf(wave_sum(sq) * inv_n + p.eps);
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) {
+      const int ch = lane + 64 * j;
+      if (ch >= n_chunks) break;
+      float y[8];
+      unpack<E>(raw[j], y);
+      const f32x4 w[2] = {*reinterpret_cast<const f32x4*>(affine + 4 * ch),
+                          *reinterpret_cast<const f32x4*>(affine + 4 * (n_chunks + ch))};
+      f32x4 bias[2];
+      if (kBias) {
+        bias[0] = *reinterpret_cast<const f32x4*>(affine + 4 * (2 * n_chunks + ch));
+        bias[1] = *reinterpret_cast<const f32x4*>(affine + 4 * (3 * n_chunks + ch));
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        y[e] = (y[e] - mu) * r * w[e >> 2][e & 3];
+        if (kBias) y[e] += bias[e >> 2][e & 3];
+      }
+      turn<kInter, false>(y, c, s);
+      store_row<kInter>(dst + j * h_step * q.y_sh, l, p.dim, pack<E>(y));
+    }
+  }
+}
+
+// ---- norm over all heads of a token, backward ----
+// One workgroup per token and tensor at a time; a thread holds kChunks groups of 8 elements, all at
+// the same place of their heads (the workgroup's size is a multiple of a row's lanes), and their
+// weights across tokens. The next token's rows are loaded before the sums of the current one,
+// which wait at a barrier.
+template <int kChunks, typename E, int kNorm, bool kInter, bool kBias>
+__global__ __launch_bounds__(kThreads) void norm_rope_token_bwd_kernel(RopeParams p) {
   const int which = blockIdx.y;
   const RopeTensor q = p.t[which];
   const int lanes = p.dim / 8;
@@ -308,23 +396,18 @@ __global__ __launch_bounds__(kThreads) void norm_rope_token_kernel(RopeParams p)
   const float inv_n = 1.f / (p.heads * p.dim);
   const int wave = threadIdx.x >> 6;
   const int n_waves = blockDim.x >> 6;
+  const int l = threadIdx.x % lanes;
+  const int h0 = threadIdx.x / lanes, h_step = blockDim.x / lanes;
 
-  int h[kChunks], l[kChunks];
   bool ok[kChunks];
-  float w[kChunks][8], bias[kChunks][8];
+  float w[kChunks][8];
   float aw[kChunks][8] = {}, ab[kChunks][8] = {};
 #pragma unroll
   for (int j = 0; j < kChunks; ++j) {
-    const int ch = threadIdx.x + j * blockDim.x;
-    ok[j] = ch < n_chunks;
-    h[j] = ok[j] ? ch / lanes : 0;
-    l[j] = ok[j] ? ch % lanes : 0;
+    ok[j] = static_cast<int>(threadIdx.x + j * blockDim.x) < n_chunks;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int i = h[j] * p.dim + col_of<kInter>(l[j], e, p.dim);
-      w[j][e] = ok[j] ? affine_at(q.w, p.w_type, i, 1.f) : 0.f;
-      bias[j][e] = !kBwd && ok[j] ? affine_at(q.b, p.w_type, i, 0.f) : 0.f;
-    }
+    for (int e = 0; e < 8; ++e)
+      w[j][e] = ok[j] ? affine_at(q.w, p.w_type, (h0 + j * h_step) * p.dim + col_of<kInter>(l, e, p.dim), 1.f) : 0.f;
   }
 
   __shared__ float red[2][3][kWaves];
@@ -349,21 +432,39 @@ __global__ __launch_bounds__(kThreads) void norm_rope_token_kernel(RopeParams p)
     turn_no ^= 1;
   };
 
-  for (int64_t item = blockIdx.x; item < static_cast<int64_t>(p.batch) * q.len; item += gridDim.x) {
+  const int64_t items = static_cast<int64_t>(p.batch) * q.len;
+  u32x4 xn[kChunks], gn[kChunks];
+  float cn[4], sn[4];
+  auto load = [&](int64_t item) {
     const int b = static_cast<int>(item / q.len);
     const int token = static_cast<int>(item % q.len);
-    float x[kChunks][8], g[kChunks][8], c[kChunks][4], s[kChunks][4];
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
-      u32x4 xv = u32x4{0, 0, 0, 0}, gv = xv;
+      xn[j] = gn[j] = u32x4{0, 0, 0, 0};
+      const int h = h0 + j * h_step;
       if (ok[j]) {
-        xv = load_row<kInter>(q.x + b * q.x_sb + h[j] * q.x_sh + token * q.x_ss, l[j], p.dim);
-        if (kBwd) gv = load_row<kInter>(q.dy + b * q.d_sb + h[j] * q.d_sh + token * q.d_ss, l[j], p.dim);
+        xn[j] = load_row<kInter>(q.x + b * q.x_sb + h * q.x_sh + token * q.x_ss, l, p.dim);
+        gn[j] = load_row<kInter>(q.dy + b * q.d_sb + h * q.d_sh + token * q.d_ss, l, p.dim);
       }
-      load_angles<kInter>(p, b, token, l[j], c[j], s[j]);
-      unpack<E>(xv, x[j]);
-      if (kBwd) unpack<E>(gv, g[j]);
     }
+    load_angles<kInter>(p, b, token, l, cn, sn);
+  };
+  if (blockIdx.x < items) load(blockIdx.x);
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int b = static_cast<int>(item / q.len);
+    const int token = static_cast<int>(item % q.len);
+    float x[kChunks][8], g[kChunks][8], c[4], s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[i] = cn[i];
+      s[i] = sn[i];
+    }
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) {
+      unpack<E>(xn[j], x[j]);
+      unpack<E>(gn[j], g[j]);
+    }
+    if (item + gridDim.x < items) load(item + gridDim.x);
     if (kNorm == kLayer) {
       float v[3] = {};
 #pragma unroll
@@ -380,53 +481,45 @@ __global__ __launch_bounds__(kThreads) void norm_rope_token_kernel(RopeParams p)
     float v[3] = {};
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
-      if (kBwd) turn<kInter, true>(g[j], c[j], s[j]);
+      turn<kInter, true>(g[j], c, s);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
+        const float d = g[j][e] * w[j][e];
         v[0] += x[j][e] * x[j][e];
-        if (kBwd) {
-          const float d = g[j][e] * w[j][e];
-          v[1] += d * x[j][e];
-          v[2] += d;
-        }
+        v[1] += d * x[j][e];
+        v[2] += d;
       }
     }
-    block_sum(v, kBwd ? (kNorm == kLayer ? 3 : 2) : 1);
+    block_sum(v, kNorm == kLayer ? 3 : 2);
     const float r = rsqrtf(v[0] * inv_n + p.eps);
-    const float m2 = kBwd ? v[1] * inv_n * r : 0.f;                        // mean(d x^)
-    const float m1 = kBwd && kNorm == kLayer ? v[2] * inv_n : 0.f;         // mean(d)
+    const float m2 = v[1] * inv_n * r;                      // mean(d x^)
+    const float m1 = kNorm == kLayer ? v[2] * inv_n : 0.f;  // mean(d)
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
       if (!ok[j]) continue;
+      const int h = h0 + j * h_step;
       float y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float n = x[j][e] * r;
-        if (kBwd) {
-          aw[j][e] += g[j][e] * n;
-          ab[j][e] += g[j][e];
-          y[e] = r * (g[j][e] * w[j][e] - n * m2 - m1);
-        } else {
-          y[e] = n * w[j][e] + bias[j][e];
-        }
+        aw[j][e] += g[j][e] * n;
+        if (kBias) ab[j][e] += g[j][e];
+        y[e] = r * (g[j][e] * w[j][e] - n * m2 - m1);
       }
-      if (!kBwd) turn<kInter, false>(y, c[j], s[j]);
-      store_row<kInter>(q.y + b * q.y_sb + h[j] * q.y_sh + token * q.y_ss, l[j], p.dim, pack<E>(y));
+      store_row<kInter>(q.y + b * q.y_sb + h * q.y_sh + token * q.y_ss, l, p.dim, pack<E>(y));
     }
   }
 
-  if constexpr (kBwd) {
-    if (p.partial == nullptr) return;
-    const int64_t n = static_cast<int64_t>(p.heads) * p.dim;
+  if (p.partial == nullptr) return;
+  const int64_t n = static_cast<int64_t>(p.heads) * p.dim;
 #pragma unroll
-    for (int j = 0; j < kChunks; ++j) {
-      if (!ok[j]) continue;
+  for (int j = 0; j < kChunks; ++j) {
+    if (!ok[j]) continue;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int64_t i = h[j] * p.dim + col_of<kInter>(l[j], e, p.dim);
-        p.partial[((which * 2) * static_cast<int64_t>(gridDim.x) + blockIdx.x) * n + i] = aw[j][e];
-        p.partial[((which * 2 + 1) * static_cast<int64_t>(gridDim.x) + blockIdx.x) * n + i] = ab[j][e];
-      }
+    for (int e = 0; e < 8; ++e) {
+      const int64_t i = (h0 + j * h_step) * p.dim + col_of<kInter>(l, e, p.dim);
+      p.partial[((which * 2) * static_cast<int64_t>(gridDim.x) + blockIdx.x) * n + i] = aw[j][e];
+      if (kBias) p.partial[((which * 2 + 1) * static_cast<int64_t>(gridDim.x) + blockIdx.x) * n + i] = ab[j][e];
     }
   }
 }
@@ -447,9 +540,18 @@ __global__ __launch_bounds__(1024) void norm_rope_sum_kernel(SumParams p) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int col = blockIdx.x * 64 + lane;
   double v = 0.0;
-  if (col < p.n)
-    for (int r = wave; r < p.records; r += 16)
-      v += p.partial[(static_cast<int64_t>(slot) * p.records + r) * p.n + col];
+  if (col < p.n) {
+    const float* at = p.partial + static_cast<int64_t>(slot) * p.records * p.n + col;
+    int r = wave;
+    for (; r + 7 * 16 < p.records; r += 8 * 16) {  // eight loads in flight
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = at[static_cast<int64_t>(r + 16 * i) * p.n];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v += x[i];
+    }
+    for (; r < p.records; r += 16) v += at[static_cast<int64_t>(r) * p.n];
+  }
   red[wave][lane] = v;
   __syncthreads();
   if (wave == 0 && col < p.n) {
@@ -485,20 +587,44 @@ int64_t groups_of(const RopeParams& p, int across) {
   return (p.items + kWaves - 1) / kWaves;
 }
 
-template <typename E, int kNorm, bool kInter, bool kBwd>
-void launch_across(const RopeParams& p, int groups, hipStream_t st) {
+template <typename E, int kNorm, bool kInter, bool kBias>
+void launch_wave(const RopeParams& p, int groups, hipStream_t st) {
+  const int chunks = p.heads * (p.dim / 8);
+  const int per = (chunks + 63) / 64;
+  const dim3 grid(groups, 2), block(kThreads);
+  const unsigned lds = static_cast<unsigned>(chunks) * 32u * (kBias ? 2u : 1u);  // at most 64 KB
+  if (per <= 3)
+    hipLaunchKernelGGL((norm_rope_wave_kernel<3, E, kNorm, kInter, kBias>), grid, block, lds, st, p);
+  else if (per <= 6)
+    hipLaunchKernelGGL((norm_rope_wave_kernel<6, E, kNorm, kInter, kBias>), grid, block, lds, st, p);
+  else if (per <= 10)
+    hipLaunchKernelGGL((norm_rope_wave_kernel<10, E, kNorm, kInter, kBias>), grid, block, lds, st, p);
+  else
+    hipLaunchKernelGGL((norm_rope_wave_kernel<16, E, kNorm, kInter, kBias>), grid, block, lds, st, p);
+}
+
+template <typename E, int kNorm, bool kInter, bool kBias>
+void launch_token_bwd(const RopeParams& p, int groups, hipStream_t st) {
   const int chunks = p.heads * (p.dim / 8);
   const int per = (chunks + kThreads - 1) / kThreads;
   const int threads = ((chunks + per - 1) / per + 63) / 64 * 64;
   const dim3 grid(groups, 2), block(threads);
   if (per == 1)
-    hipLaunchKernelGGL((norm_rope_token_kernel<1, E, kNorm, kInter, kBwd>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((norm_rope_token_bwd_kernel<1, E, kNorm, kInter, kBias>), grid, block, 0, st, p);
   else if (per == 2)
-    hipLaunchKernelGGL((norm_rope_token_kernel<2, E, kNorm, kInter, kBwd>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((norm_rope_token_bwd_kernel<2, E, kNorm, kInter, kBias>), grid, block, 0, st, p);
   else if (per == 3)
-    hipLaunchKernelGGL((norm_rope_token_kernel<3, E, kNorm, kInter, kBwd>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((norm_rope_token_bwd_kernel<3, E, kNorm, kInter, kBias>), grid, block, 0, st, p);
   else
-    hipLaunchKernelGGL((norm_rope_token_kernel<4, E, kNorm, kInter, kBwd>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((norm_rope_token_bwd_kernel<4, E, kNorm, kInter, kBias>), grid, block, 0, st, p);
+}
+
+template <typename E, int kNorm, bool kInter, bool kBwd>
+void launch_across(const RopeParams& p, int groups, hipStream_t st) {
+  if constexpr (kBwd)
+    p.has_bias ? launch_token_bwd<E, kNorm, kInter, true>(p, groups, st) : launch_token_bwd<E, kNorm, kInter, false>(p, groups, st);
+  else
+    p.has_bias ? launch_wave<E, kNorm, kInter, true>(p, groups, st) : launch_wave<E, kNorm, kInter, false>(p, groups, st);
 }
 
 template <typename E, int kNorm, bool kInter, bool kBwd>
@@ -580,6 +706,7 @@ int rope_setup(const char* what, RopeParams& p, int batch, int heads, int q_len,
   p.tokens = q_len > k_len ? q_len : k_len;
   p.t[0].w = qw;
   p.t[1].w = kw;
+  p.has_bias = qb != nullptr || kb != nullptr;
   p.t[0].b = qb;
   p.t[1].b = kb;
   p.t[0].len = q_len;
@@ -632,9 +759,11 @@ extern "C" int moddit_qk_norm_rope(const void* q, const void* k, void* q_out, vo
   }
   p.token_major = q_strides[1] < q_strides[2];
   plan_heads(p, head_dim);
-  // a workgroup of the token kernel walks several tokens: its weights stay in registers
   int64_t groups = groups_of(p, across_heads);
-  if (across_heads && groups > 4096) groups = 4096;
+  if (across_heads) {  // a wave walks several tokens, so that the weights are read to LDS seldom
+    groups = (groups + kWaves - 1) / kWaves;
+    if (groups > 1280) groups = 1280;
+  }
   MODDIT_CHECK_ARG(groups <= 0x7fffffff, "qk_norm_rope: too many tokens");
   launch_rope<false>(p, dtype, norm, across_heads, interleaved, static_cast<int>(groups), as_stream(stream));
   MODDIT_CHECK_LAUNCH("qk_norm_rope");
@@ -703,6 +832,7 @@ extern "C" int moddit_qk_norm_rope_bwd(const void* q, const void* k, const void*
                      "qk_norm_rope_bwd: workspace of %lld floats, %lld needed", static_cast<long long>(workspace_floats),
                      static_cast<long long>(4 * groups * row));
     p.partial = workspace;
+    p.has_bias = dq_bias != nullptr || dk_bias != nullptr;
   }
   hipStream_t st = as_stream(stream);
   launch_rope<true>(p, dtype, norm, across_heads, interleaved, groups, st);

@@ -364,11 +364,14 @@ int moddit_refresh_merge(const void* prev, const void* cur, const uint8_t* mask,
  * them in its range), each output rounded once. Rows with lse = -inf attend to nothing: they get
  * dq = 0 and add nothing. Sums are formed in a fixed order: results repeat bit for bit.
  * q_len or kv_len may be 0 (the other side's gradients are then zeros). batch * heads <= 65535.
- * `workspace`: moddit_attention_bwd_workspace_bytes bytes, 16-byte aligned, one per call in
- * flight. No gradient may overlap an input.
+ * `workspace`: moddit_attention_bwd_workspace_bytes bytes (cap = key_cap = 0 for this call, the
+ * lists' capacities for moddit_block_sparse_bwd), 16-byte aligned, one per call in flight: row
+ * statistics, and fp32 partial sums of launches with few tiles, whose streamed rows are shared
+ * among workgroups. No gradient may overlap an input.
  */
 int64_t moddit_attention_bwd_workspace_bytes(int batch, int heads, int q_len, int kv_len,
-                                             int head_dim, int dtype, int grid_origin);
+                                             int head_dim, int dtype, int grid_origin, int cap,
+                                             int key_cap);
 int moddit_flash_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse,
                      const void* grad_o, const float* grad_lse, void* dq, void* dk, void* dv,
                      int batch, int heads, int q_len, int kv_len, int head_dim,

@@ -70,7 +70,7 @@ _SIGNATURES = {
                                     _vp, _vp, _vp, _i, _i, _vp]),
     "moddit_mask_to_tiles": (_i, [_vp, _i, _i, _i, ctypes.c_int64, ctypes.c_int64, _i, _i, _i,
                                   _vp, _vp, _i, _i, _vp]),
-    "moddit_attention_bwd_workspace_bytes": (ctypes.c_int64, [_i] * 7),
+    "moddit_attention_bwd_workspace_bytes": (ctypes.c_int64, [_i] * 9),
     "moddit_flash_bwd": (_i, [_vp] * 10 + [_i] * 5 + [_c_i64p] * 8 + [_f, _i, _vp, ctypes.c_int64, _vp]),
     "moddit_block_sparse_bwd": (_i, [_vp] * 10 + [_i] * 5 + [_c_i64p] * 8 + [_f, _i] +
                                 [_vp, _vp, _i, _i] * 2 + [_i, _vp, ctypes.c_int64, _vp]),

@@ -97,6 +97,11 @@ struct BwdParams {
   const int32_t* counts;
   const int32_t* entries;
   int cap;
+  const int32_t* order;  // workgroup -> tile, long lists first (order_kernel); or null
+  // split streamed range: n_split workgroups per tile leave their fp32 sums in
+  // part [tile][piece][dQ, or dK and dV][128][D]
+  int n_split;
+  float* part;
 };
 
 // ---- row statistics ----
@@ -227,7 +232,7 @@ __device__ __forceinline__ int ds_exponent(const float* maxima, int n, float (*r
   return e < -100 ? -100 : (e > 100 ? 100 : e);
 }
 
-template <int D, typename E, bool kKeys, bool kSparse>
+template <int D, typename E, bool kKeys, bool kSparse, bool kSplit>
 __global__ __launch_bounds__(kThreads, 2) void attention_bwd_kernel(BwdParams p) {
   using L = BwdLds<D, kKeys>;
   using V8 = typename E::vec8;
@@ -242,7 +247,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_bwd_kernel(BwdParams p)
   const int g = lane >> 4;
   const int c16 = lane & 15;
 
-  const int tile = xcd_remap(blockIdx.x, gridDim.x, p.xcd_run);
+  int tile = kSplit ? blockIdx.x / p.n_split : xcd_remap(blockIdx.x, gridDim.x, p.xcd_run);
+  if (kSparse && !kSplit && p.order != nullptr) tile = p.order[tile];
   const int ot = tile % p.n_tiles;
   const int bh = tile / p.n_tiles;
   const int b = bh / p.heads;
@@ -255,6 +261,16 @@ __global__ __launch_bounds__(kThreads, 2) void attention_bwd_kernel(BwdParams p)
     n_iter = p.counts[slot];
     n_iter = n_iter < 0 ? 0 : (n_iter < p.cap ? n_iter : p.cap);
     list = p.entries + slot * p.cap;
+  }
+  int it0 = 0;  // first streamed tile (dense) of this workgroup's piece
+  if constexpr (kSplit) {
+    const int piece = blockIdx.x - tile * p.n_split;
+    const int first = static_cast<int>(static_cast<int64_t>(n_iter) * piece / p.n_split);
+    n_iter = static_cast<int>(static_cast<int64_t>(n_iter) * (piece + 1) / p.n_split) - first;
+    if (kSparse)
+      list += first;
+    else
+      it0 = first;
   }
   const int first_row = p.origin + ot * kBM + __builtin_amdgcn_readfirstlane(wave) * 32;
   const int wbit = first_row < p.own_len && first_row + 31 >= 0 ? 1 << (wave >> 1) : 0;
@@ -366,7 +382,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_bwd_kernel(BwdParams p)
     flags = (st >= 0 && st < p.n_str_tiles) ? (e & 3) : 0;  // as in the forward
     st = st < 0 ? 0 : (st < p.n_str_tiles ? st : p.n_str_tiles - 1);
   };
-  auto entry = [&](int i) -> int { return kSparse ? list[i] : ((i << 2) | 3); };
+  auto entry = [&](int i) -> int { return kSparse ? list[i] : (((it0 + i) << 2) | 3); };
   auto tr_operand = [&](const unsigned char* a) -> V8 {
     const s16x4 lo = lds_read_tr16(a);
     const s16x4 hi = lds_read_tr16(a + 16 * L::kRowBytes);
@@ -484,6 +500,19 @@ __global__ __launch_bounds__(kThreads, 2) void attention_bwd_kernel(BwdParams p)
     flags = flags1;
   }
 
+  if constexpr (kSplit) {
+    float* part = p.part + static_cast<int64_t>(blockIdx.x) * (kKeys ? 2 : 1) * kBM * D;
+#pragma unroll
+    for (int qq = 0; qq < 2; ++qq) {
+      float* r = part + (wave * 32 + 16 * qq + c16) * D + 4 * g;
+#pragma unroll
+      for (int db = 0; db < kDB; ++db) {
+        *reinterpret_cast<f32x4*>(r + db * 16) = acc1[db][qq] * out1_scale;
+        if constexpr (kKeys) *reinterpret_cast<f32x4*>(r + kBM * D + db * 16) = acc2[db][qq] * (kHalf ? 0x1p-15f : 1.f);
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int qq = 0; qq < 2; ++qq) {
     const int row = row0 + 16 * qq;
@@ -511,10 +540,127 @@ __global__ __launch_bounds__(kThreads, 2) void attention_bwd_kernel(BwdParams p)
   }
 }
 
-template <int D, typename E, bool kKeys, bool kSparse>
+// The pieces of a tile -> its rows, added in piece order. A workgroup takes kCombineRows rows of
+// one tile and tensor, a thread four of its columns. Bound by reading the partials back, mostly
+// from L2 and the last-level cache.
+constexpr int kCombineRows = 16;
+
+template <int D, typename E, bool kKeys>
+__global__ __launch_bounds__(kThreads) void combine_bwd_kernel(BwdParams p) {
+  constexpr int kCols = D / 4;
+  constexpr int kTensors = kKeys ? 2 : 1;
+  const int tile = blockIdx.x / (kBM / kCombineRows);
+  const int r_first = (blockIdx.x % (kBM / kCombineRows)) * kCombineRows;
+  const bool second = kKeys && blockIdx.y == 1;
+  const int ot = tile % p.n_tiles;
+  const int bh = tile / p.n_tiles;
+  const int b = bh / p.heads, h = bh % p.heads;
+  const int d = (threadIdx.x % kCols) * 4;
+  for (int r = r_first + threadIdx.x / kCols; r < r_first + kCombineRows; r += kThreads / kCols) {
+    const int row = p.origin + ot * kBM + r;
+    if (row < 0 || row >= p.own_len) continue;
+    const float* at = p.part + ((static_cast<int64_t>(tile) * p.n_split * kTensors + second) * kBM + r) * D + d;
+    f32x4 x = f32x4{};
+    for (int i = 0; i < p.n_split; ++i) x += *reinterpret_cast<const f32x4*>(at + static_cast<int64_t>(i) * kTensors * kBM * D);
+    u32x2 w;
+    w.x = pack2(E::from_float(x[0]), E::from_float(x[1]));
+    w.y = pack2(E::from_float(x[2]), E::from_float(x[3]));
+    uint16_t* o = second ? p.out2 + b * p.o2_sb + h * p.o2_sh + row * p.o2_ss
+                         : p.out1 + b * p.o1_sb + h * p.o1_sh + row * p.o1_ss;
+    *reinterpret_cast<u32x2*>(o + d) = w;
+  }
+}
+
+// ---- order of tiles whose lists differ in length ----
+// A full column of a mask (text keys, a kept line) gives a key tile many times the mean of
+// queries; started last, it runs alone at the end. The tiles of each pass in order of how far
+// their lists lie above the mean, kept in their natural order within a class, so that neighbours
+// still share what they stream. One workgroup per pass.
+struct OrderParams {
+  const int32_t* counts[2];
+  int32_t* order[2];
+  int tiles[2];  // heads * tiles of a head: every batch follows the same lists
+  int batch;
+};
+
+constexpr int kClasses = 6;
+
+__global__ __launch_bounds__(1024) void order_kernel(OrderParams p) {
+  __shared__ int hist[kClasses][1024];
+  __shared__ long long total;
+  __shared__ int start[kClasses];
+  const int pass = blockIdx.x;
+  const int n = p.tiles[pass];
+  const int32_t* counts = p.counts[pass];
+  const int tid = threadIdx.x;
+  const int per = (n + 1023) / 1024;
+  const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
+  int sum = 0;
+  for (int i = i0; i < i1; ++i) sum += counts[i];
+  hist[0][tid] = sum;
+  __syncthreads();
+  if (tid == 0) {
+    long long t = 0;
+    for (int i = 0; i < 1024; ++i) t += hist[0][i];
+    total = t;
+  }
+  __syncthreads();
+  const float mean = static_cast<float>(total) / n;
+  auto class_of = [&](int c) {
+    const float r = c / mean;
+    return r >= 4.f ? 0 : r >= 2.8f ? 1 : r >= 2.f ? 2 : r >= 1.4f ? 3 : r >= 0.7f ? 4 : 5;
+  };
+  int mine[kClasses] = {};
+  for (int i = i0; i < i1; ++i) {
+    const int c = class_of(counts[i]);
+#pragma unroll
+    for (int k = 0; k < kClasses; ++k) mine[k] += c == k;
+  }
+#pragma unroll
+  for (int k = 0; k < kClasses; ++k) hist[k][tid] = mine[k];
+  __syncthreads();
+  // exclusive prefix of each class over the threads: wave k scans class k
+  if (tid / 64 < kClasses) {
+    const int k = tid / 64, lane = tid % 64;
+    int run = 0;
+    for (int j = 0; j < 1024; j += 64) {
+      const int v = hist[k][j + lane];
+      int x = v;
+#pragma unroll
+      for (int m = 1; m < 64; m *= 2) {
+        const int y = __shfl_up(x, m);
+        if (lane >= m) x += y;
+      }
+      hist[k][j + lane] = run + x - v;
+      run += __shfl(x, 63);
+    }
+    if (lane == 0) start[k] = run;
+  }
+  __syncthreads();
+  int at[kClasses];
+  int before = 0;
+#pragma unroll
+  for (int k = 0; k < kClasses; ++k) {
+    at[k] = before * p.batch + hist[k][tid] * p.batch;
+    before += start[k];
+  }
+  for (int i = i0; i < i1; ++i) {
+    const int c = class_of(counts[i]);
+    int to = 0;
+#pragma unroll
+    for (int k = 0; k < kClasses; ++k)
+      if (c == k) {
+        to = at[k];
+        at[k] += p.batch;
+      }
+    for (int b = 0; b < p.batch; ++b) p.order[pass][to + b] = b * n + i;
+  }
+}
+
+template <int D, typename E, bool kKeys, bool kSparse, bool kSplit>
 int launch_pass(const BwdParams& p, int batch, hipStream_t st) {
   constexpr int kLds = BwdLds<D, kKeys>::kTotal;
-  auto kernel = attention_bwd_kernel<D, E, kKeys, kSparse>;
+  auto kernel = attention_bwd_kernel<D, E, kKeys, kSparse, kSplit>;
   static LaunchSetup once;
   if (set_dynamic_lds_once(once, reinterpret_cast<const void*>(kernel), kLds) != hipSuccess) {
     set_error("attention_bwd: cannot reserve %d bytes of LDS", kLds);
@@ -522,13 +668,23 @@ int launch_pass(const BwdParams& p, int batch, hipStream_t st) {
   }
   const int64_t tiles = static_cast<int64_t>(batch) * p.heads * p.n_tiles;
   if (tiles == 0) return MODDIT_OK;
-  if (tiles > 0x7fffffff) {
-    set_error("attention_bwd: too many tiles (%lld)", static_cast<long long>(tiles));
-    return MODDIT_EINVAL;
-  }
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles)), dim3(kThreads), kLds, st, p);
+  const int64_t grid = kSplit ? tiles * p.n_split : tiles;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), kLds, st, p);
   MODDIT_CHECK_LAUNCH("attention_bwd");
+  if constexpr (kSplit) {
+    hipLaunchKernelGGL((combine_bwd_kernel<D, E, kKeys>), dim3(static_cast<unsigned>(tiles * (kBM / kCombineRows)), kKeys ? 2 : 1),
+                       dim3(kThreads), 0, st, p);
+    MODDIT_CHECK_LAUNCH("attention_bwd (combine)");
+  }
   return MODDIT_OK;
+}
+
+template <int D, typename E, bool kKeys>
+int launch_side(const BwdParams& p, int batch, hipStream_t st) {
+  const bool sparse = p.counts != nullptr;
+  if (p.n_split > 1)
+    return sparse ? launch_pass<D, E, kKeys, true, true>(p, batch, st) : launch_pass<D, E, kKeys, false, true>(p, batch, st);
+  return sparse ? launch_pass<D, E, kKeys, true, false>(p, batch, st) : launch_pass<D, E, kKeys, false, false>(p, batch, st);
 }
 
 template <int D, typename E>
@@ -539,20 +695,87 @@ int launch_bwd(const StatsParams& sp, const BwdParams& dq, const BwdParams& dkv,
     hipLaunchKernelGGL((stats_kernel<D, E, kMax>), dim3(blocks, batch * sp.heads), dim3(kThreads), 0, st, sp);
     MODDIT_CHECK_LAUNCH("attention_bwd (row statistics)");
   }
-  const bool sparse = dq.counts != nullptr;
-  if (const int rc = sparse ? launch_pass<D, E, false, true>(dq, batch, st) : launch_pass<D, E, false, false>(dq, batch, st)) return rc;
-  return sparse ? launch_pass<D, E, true, true>(dkv, batch, st) : launch_pass<D, E, true, false>(dkv, batch, st);
+  if (dq.order != nullptr) {
+    const OrderParams op{{dq.counts, dkv.counts}, {const_cast<int32_t*>(dq.order), const_cast<int32_t*>(dkv.order)},
+                         {dq.heads * dq.n_tiles, dkv.heads * dkv.n_tiles}, batch};
+    hipLaunchKernelGGL(order_kernel, dim3(2), dim3(1024), 0, st, op);
+    MODDIT_CHECK_LAUNCH("attention_bwd (order)");
+  }
+  if (const int rc = launch_side<D, E, false>(dq, batch, st)) return rc;
+  return launch_side<D, E, true>(dkv, batch, st);
 }
 
-// Blocks of 64 grid rows (whole tiles of 128) and of maxima, and the floats of both.
+// ---- sizes ----
+// Blocks of 64 grid rows (whole tiles of 128) and of maxima.
 int64_t stat_blocks_of(int q_len, int origin) { return (static_cast<int64_t>(q_len) - origin + kBM - 1) / kBM * 2; }
 int64_t maxima_of(int q_len, int kv_len, int origin) {
   const int64_t a = stat_blocks_of(q_len, origin), b = (static_cast<int64_t>(kv_len) + 63) / 64;
   return a > b ? a : b;
 }
-int64_t bwd_workspace_floats(int batch, int heads, int q_len, int kv_len, int dtype, int origin) {
-  return static_cast<int64_t>(batch) * heads *
-         (stat_blocks_of(q_len, origin) * 128 + (dtype == MODDIT_FP16 ? maxima_of(q_len, kv_len, origin) * 4 : 0));
+
+// How many workgroups share a tile's streamed range: see split_for in attention.hip; here the
+// partial sums are dQ's, or dK's and dV's.
+constexpr int kMaxSplit = 64;
+
+double cu_step_us(int head_dim, bool keys, int64_t k) {
+  constexpr double t128[2][2] = {{1.63, 2.6}, {2.3, 3.64}}, t64[2][3] = {{0.9, 1.2, 1.6}, {1.2, 1.6, 2.2}};
+  if (head_dim == 128) return k <= 2 ? t128[keys][k - 1] : t128[keys][1] / 2 * k;
+  return k <= 3 ? t64[keys][k - 1] : t64[keys][2] / 3 * k;
+}
+
+int split_for(int64_t tiles, int64_t steps, int head_dim, bool keys) {
+  constexpr double kCus = 256, kFixedSteps = 4, kLaunchUs = 5.0, kPartialBytesPerUs = 4.0e6;
+  int best = 1;
+  double best_us = 0.0;
+  if (tiles == 0) return 1;
+  for (int s = 1; s <= kMaxSplit; ++s) {
+    if (s > 1 && steps < 4 * static_cast<int64_t>(s)) break;
+    const int64_t per_cu = static_cast<int64_t>((tiles * s + kCus - 1) / kCus);
+    double us = cu_step_us(head_dim, keys, per_cu) * (static_cast<double>(steps) / s + kFixedSteps);
+    if (s > 1) us += kLaunchUs + tiles * s * (kBM * head_dim * 8.0 * (keys ? 2 : 1)) / kPartialBytesPerUs;
+    if (s == 1 || us < 0.97 * best_us) {
+      best = s;
+      best_us = us;
+    }
+  }
+  return best;
+}
+
+constexpr int64_t kResident = 512;  // workgroups that run at once at least: fewer tiles need no order
+
+struct BwdPlan {
+  int64_t stat_blocks, n_maxima, tiles[2];
+  int n_split[2];
+  bool order;
+  int64_t stats, maxima, orders, parts[2], total;  // floats, each from a multiple of 4
+};
+
+// What a call of these sizes runs and keeps in its workspace. cap, key_cap: 0 for dense calls; a
+// block-sparse list is taken to hold a quarter of its capacity.
+BwdPlan plan_bwd(int batch, int heads, int q_len, int kv_len, int head_dim, int dtype, int origin, int cap, int key_cap) {
+  BwdPlan p;
+  const int64_t bh = static_cast<int64_t>(batch) * heads;
+  auto tiles_of = [&](int len) { return len > 0 ? (static_cast<int64_t>(len) - origin + kBM - 1) / kBM : 0; };
+  auto steps_of = [&](int len) { return len > 0 ? (static_cast<int64_t>(len) - origin + kBN - 1) / kBN : 0; };
+  p.stat_blocks = stat_blocks_of(q_len, origin);
+  p.n_maxima = dtype == MODDIT_FP16 ? maxima_of(q_len, kv_len, origin) : 0;
+  p.tiles[0] = tiles_of(q_len);
+  p.tiles[1] = tiles_of(kv_len);
+  const int64_t steps[2] = {cap > 0 ? cap / 4 : steps_of(kv_len), key_cap > 0 ? key_cap / 4 : steps_of(q_len)};
+  for (int i = 0; i < 2; ++i) p.n_split[i] = split_for(bh * p.tiles[i], steps[i], head_dim, i == 1);
+  p.order = cap > 0 && bh * (p.tiles[0] > p.tiles[1] ? p.tiles[0] : p.tiles[1]) > kResident;
+  auto up4 = [](int64_t x) { return (x + 3) / 4 * 4; };
+  p.stats = 0;
+  p.maxima = p.stats + bh * p.stat_blocks * 128;
+  p.orders = p.maxima + bh * p.n_maxima * 4;
+  int64_t at = p.orders + (p.order ? up4(bh * (p.tiles[0] + p.tiles[1])) : 0);
+  for (int i = 0; i < 2; ++i) {
+    p.parts[i] = at;
+    // the passes run one after the other, each with its combine: they share the room
+    const int64_t n = p.n_split[i] > 1 ? bh * p.tiles[i] * p.n_split[i] * kBM * head_dim * (i + 1) : 0;
+    p.total = i == 0 ? at + n : (at + n > p.total ? at + n : p.total);
+  }
+  return p;
 }
 
 struct BwdArgs {
@@ -610,7 +833,13 @@ int bwd_entry(const BwdArgs& a, moddit_stream_t stream) {
                    "attention_bwd: null tensor pointer");
   const void* all[8] = {a.q, a.k, a.v, a.o, a.d, a.dq, a.dk, a.dv};
   for (const void* t : all) MODDIT_CHECK_ARG(aligned16(t), "attention_bwd: tensors must be 16-byte aligned");
-  const int64_t need = bwd_workspace_floats(a.batch, a.heads, a.q_len, a.kv_len, a.dtype, a.origin) * 4;
+  const bool lists = sparse && a.q_len > 0 && a.kv_len > 0;  // an empty side's lists name no row
+  const BwdPlan plan = plan_bwd(a.batch, a.heads, a.q_len, a.kv_len, a.head_dim, a.dtype, a.origin, lists ? a.cap : 0,
+                                lists ? a.key_cap : 0);
+  const int64_t need = plan.total * 4;
+  for (int i = 0; i < 2; ++i)
+    MODDIT_CHECK_ARG(plan.tiles[i] * a.batch * a.heads * (kBM / kCombineRows) * plan.n_split[i] <= 0x7fffffff,
+                     "attention_bwd: too many tiles");
   MODDIT_CHECK_ARG((a.workspace != nullptr || need == 0) && aligned16(a.workspace) && a.workspace_bytes >= need,
                    "attention_bwd: a 16-byte aligned workspace of %lld bytes is needed, got %lld",
                    static_cast<long long>(need), static_cast<long long>(a.workspace_bytes));
@@ -636,10 +865,11 @@ int bwd_entry(const BwdArgs& a, moddit_stream_t stream) {
   sp.q_len = a.q_len;
   sp.kv_len = a.kv_len;
   sp.origin = a.origin;
-  sp.stat_blocks = static_cast<int>(stat_blocks_of(a.q_len, a.origin));
-  sp.n_maxima = static_cast<int>(maxima_of(a.q_len, a.kv_len, a.origin));
-  sp.stats = static_cast<float*>(a.workspace);
-  sp.maxima = sp.stats + static_cast<int64_t>(a.batch) * a.heads * sp.stat_blocks * 128;
+  float* const ws = static_cast<float*>(a.workspace);
+  sp.stat_blocks = static_cast<int>(plan.stat_blocks);
+  sp.n_maxima = static_cast<int>(plan.n_maxima);
+  sp.stats = ws + plan.stats;
+  sp.maxima = ws + plan.maxima;
   sp.p_exponent = a.dtype == MODDIT_FP16 ? kPExponent : 0.f;
 
   BwdParams p;
@@ -666,8 +896,13 @@ int bwd_entry(const BwdArgs& a, moddit_stream_t stream) {
   dkv.o2_sb = a.dvs[0]; dkv.o2_sh = a.dvs[1]; dkv.o2_ss = a.dvs[2];
   dq.own_len = dkv.str_len = a.q_len;
   dq.str_len = dkv.own_len = a.kv_len;
-  dq.n_tiles = a.q_len > 0 ? static_cast<int>(nq) : 0;
-  dkv.n_tiles = a.kv_len > 0 ? static_cast<int>(nk) : 0;
+  dq.n_tiles = static_cast<int>(plan.tiles[0]);
+  dkv.n_tiles = static_cast<int>(plan.tiles[1]);
+  dq.n_split = plan.n_split[0];
+  dkv.n_split = plan.n_split[1];
+  dq.part = ws + plan.parts[0];
+  dkv.part = ws + plan.parts[1];
+  dq.order = dkv.order = nullptr;
   dq.n_str_tiles = a.kv_len > 0 ? static_cast<int>((static_cast<int64_t>(a.kv_len) - a.origin + kBN - 1) / kBN) : 0;
   dkv.n_str_tiles = a.q_len > 0 ? static_cast<int>((static_cast<int64_t>(a.q_len) - a.origin + kBN - 1) / kBN) : 0;
   dq.xcd_run = xcd_run_for(static_cast<int64_t>(a.kv_len) * a.head_dim * 4);
@@ -676,14 +911,18 @@ int bwd_entry(const BwdArgs& a, moddit_stream_t stream) {
   dkv.str2_bytes = static_cast<uint32_t>(spans[1]);
   dq.str1_bytes = static_cast<uint32_t>(spans[2]);
   dq.str2_bytes = static_cast<uint32_t>(spans[3]);
-  dq.counts = a.counts;
+  dq.counts = lists ? a.counts : nullptr;
   dq.entries = a.entries;
   dq.cap = a.cap;
-  dkv.counts = a.key_counts;
+  dkv.counts = lists ? a.key_counts : nullptr;
   dkv.entries = a.key_entries;
   dkv.cap = a.key_cap;
-  // lists of a side whose counterpart is empty name no row
-  if (sparse && (a.q_len == 0 || a.kv_len == 0)) dq.counts = dkv.counts = nullptr;
+  if (plan.order) {
+    dq.order = reinterpret_cast<int32_t*>(ws + plan.orders);
+    dkv.order = dq.order + static_cast<int64_t>(a.batch) * a.heads * plan.tiles[0];
+    // dealt to the XCDs in runs: a contiguous eighth each would give one XCD all long lists
+    dq.xcd_run = dkv.xcd_run = kXcdRun;
+  }
 
   hipStream_t st = as_stream(stream);
   const bool bf = a.dtype == MODDIT_BF16;
@@ -751,10 +990,13 @@ __global__ __launch_bounds__(kThreads) void transpose_tiles_kernel(const int32_t
 }  // namespace moddit
 
 extern "C" int64_t moddit_attention_bwd_workspace_bytes(int batch, int heads, int q_len, int kv_len, int head_dim,
-                                                        int dtype, int grid_origin) {
+                                                        int dtype, int grid_origin, int cap, int key_cap) {
   using namespace moddit;
-  if (batch <= 0 || heads <= 0 || q_len < 0 || kv_len < 0 || grid_origin > 0 || grid_origin <= -kBN) return 0;
-  return bwd_workspace_floats(batch, heads, q_len, kv_len, dtype, grid_origin) * 4;
+  if (batch <= 0 || heads <= 0 || q_len < 0 || kv_len < 0 || (head_dim != 64 && head_dim != 128) || grid_origin > 0 ||
+      grid_origin <= -kBN || cap < 0 || key_cap < 0)
+    return 0;
+  if (q_len == 0 || kv_len == 0) cap = key_cap = 0;
+  return plan_bwd(batch, heads, q_len, kv_len, head_dim, dtype, grid_origin, cap, key_cap).total * 4;
 }
 
 extern "C" int moddit_flash_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse,

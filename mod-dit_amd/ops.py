@@ -291,7 +291,8 @@ def _attention_bwd(what, q, k, v, out, lse, grad_out, scale, grad_lse, tiles, ke
     lse, grad_lse = (None if t is None else t.contiguous() for t in (lse, grad_lse))
     dq, dk, dv = _empty_as(q), _empty_as(k), _empty_as(v)
     lib = _lib.load()
-    nbytes = _split_bytes("moddit_attention_bwd_workspace_bytes", B, H, Sq, Skv, D, dt, origin)
+    nbytes = _split_bytes("moddit_attention_bwd_workspace_bytes", B, H, Sq, Skv, D, dt, origin,
+                          0 if tiles is None else tiles.cap, 0 if tiles is None else key_tiles.cap)
     ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
     args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), grad_out.data_ptr(),
             _ptr(grad_lse), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, H, Sq, Skv, D,

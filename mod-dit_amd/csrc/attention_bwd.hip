@@ -233,7 +233,7 @@ __device__ __forceinline__ int ds_exponent(const float* maxima, int n, float (*r
 }
 
 template <int D, typename E, bool kKeys, bool kSparse, bool kSplit>
-__global__ __launch_bounds__(kThreads, 2) void attention_bwd_kernel(BwdParams p) {
+__global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void attention_bwd_kernel(BwdParams p) {
   using L = BwdLds<D, kKeys>;
   using V8 = typename E::vec8;
   constexpr int kKC = D / 32;  // MFMA k-steps over d
@@ -275,44 +275,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_bwd_kernel(BwdParams p)
   const int first_row = p.origin + ot * kBM + __builtin_amdgcn_readfirstlane(wave) * 32;
   const int wbit = first_row < p.own_len && first_row + 31 >= 0 ? 1 << (wave >> 1) : 0;
 
-  float ds_scale = 1.f;  // fp16, dK/dV: 2^(e - 15), from 2^15 P to 2^e dS
-  float out1_scale = p.scale;
-  int ds_exp = 0;
-  if constexpr (kHalf) {
-    ds_exp = ds_exponent(p.maxima + static_cast<int64_t>(bh) * p.n_maxima * 4, p.n_maxima,
-                         reinterpret_cast<float(*)[4]>(smem));
-    ds_scale = ldexpf(1.f, ds_exp - static_cast<int>(kPExponent));
-    out1_scale *= ldexpf(1.f, -ds_exp);
-  }
-
-  // ---- owned rows (B operands): lane holds row 16qq + c16, dims 32c + 8g.. ----
-  const int row0 = p.origin + ot * kBM + wave * 32 + c16;
-  V8 own1[2][kKC], own2[2][L::kOwn2InLds ? 1 : kKC];
-#pragma unroll
-  for (int qq = 0; qq < 2; ++qq) {
-    const int row = row0 + 16 * qq;
-    const int r = row < 0 ? 0 : (row < p.own_len ? row : p.own_len - 1);
-    const u32x4* a = reinterpret_cast<const u32x4*>(p.own1.p + b * p.own1.sb + h * p.own1.sh + r * p.own1.ss);
-    const u32x4* c = reinterpret_cast<const u32x4*>(p.own2.p + b * p.own2.sb + h * p.own2.sh + r * p.own2.ss);
-#pragma unroll
-    for (int i = 0; i < kKC; ++i) {
-      own1[qq][i] = as_vec8<V8>(a[4 * i + g]);
-      if constexpr (!L::kOwn2InLds) own2[qq][i] = as_vec8<V8>(c[4 * i + g]);
-    }
-  }
   const float* stats = p.stats + static_cast<int64_t>(bh) * p.stat_blocks * 128;
-  float nl_own[2] = {0.f, 0.f}, nd_own[2] = {0.f, 0.f};
-  if constexpr (!kKeys) {
-#pragma unroll
-    for (int qq = 0; qq < 2; ++qq) {
-      const int gr = ot * kBM + wave * 32 + 16 * qq + c16;
-      const float* s = stats + (gr >> 6) * 128 + (gr & 63);
-      nl_own[qq] = s[0] + (kHalf ? ds_exp - kPExponent : 0.f);
-      nd_own[qq] = s[64];
-    }
-  }
-  __builtin_amdgcn_s_waitcnt(0);
-
   // ---- staging, as in the forward: window w of a tile holds LDS bytes [1024 w, +1024) ----
   const u32x4 rsrc1 = raw_rsrc(p.str1.p + b * p.str1.sb + h * p.str1.sh, p.str1_bytes);
   const u32x4 rsrc2 = raw_rsrc(p.str2.p + b * p.str2.sb + h * p.str2.sh, p.str2_bytes);
@@ -355,6 +318,56 @@ __global__ __launch_bounds__(kThreads, 2) void attention_bwd_kernel(BwdParams p)
     }
   }
 
+  auto decode = [&](int e_raw, int& st, int& flags) {
+    const int e = __builtin_amdgcn_readfirstlane(e_raw);
+    st = e >> 2;
+    flags = (st >= 0 && st < p.n_str_tiles) ? (e & 3) : 0;  // as in the forward
+    st = st < 0 ? 0 : (st < p.n_str_tiles ? st : p.n_str_tiles - 1);
+  };
+  auto entry = [&](int i) -> int { return kSparse ? list[i] : (((it0 + i) << 2) | 3); };
+  // the first stage is on its way while the owned rows are read
+  int st = 0, flags = 0;
+  if (n_iter > 0) {
+    decode(entry(0), st, flags);
+    dma(st, 0, 0);
+  }
+
+  float ds_scale = 1.f;  // fp16, dK/dV: 2^(e - 15), from 2^15 P to 2^e dS
+  float out1_scale = p.scale;
+  int ds_exp = 0;
+  if constexpr (kHalf) {
+    __shared__ float red[4][4];
+    ds_exp = ds_exponent(p.maxima + static_cast<int64_t>(bh) * p.n_maxima * 4, p.n_maxima, red);
+    ds_scale = ldexpf(1.f, ds_exp - static_cast<int>(kPExponent));
+    out1_scale *= ldexpf(1.f, -ds_exp);
+  }
+
+  // ---- owned rows (B operands): lane holds row 16qq + c16, dims 32c + 8g.. ----
+  const int row0 = p.origin + ot * kBM + wave * 32 + c16;
+  V8 own1[2][kKC], own2[2][L::kOwn2InLds ? 1 : kKC];
+#pragma unroll
+  for (int qq = 0; qq < 2; ++qq) {
+    const int row = row0 + 16 * qq;
+    const int r = row < 0 ? 0 : (row < p.own_len ? row : p.own_len - 1);
+    const u32x4* a = reinterpret_cast<const u32x4*>(p.own1.p + b * p.own1.sb + h * p.own1.sh + r * p.own1.ss);
+    const u32x4* c = reinterpret_cast<const u32x4*>(p.own2.p + b * p.own2.sb + h * p.own2.sh + r * p.own2.ss);
+#pragma unroll
+    for (int i = 0; i < kKC; ++i) {
+      own1[qq][i] = as_vec8<V8>(a[4 * i + g]);
+      if constexpr (!L::kOwn2InLds) own2[qq][i] = as_vec8<V8>(c[4 * i + g]);
+    }
+  }
+  float nl_own[2] = {0.f, 0.f}, nd_own[2] = {0.f, 0.f};
+  if constexpr (!kKeys) {
+#pragma unroll
+    for (int qq = 0; qq < 2; ++qq) {
+      const int gr = ot * kBM + wave * 32 + 16 * qq + c16;
+      const float* s = stats + (gr >> 6) * 128 + (gr & 63);
+      nl_own[qq] = s[0] + (kHalf ? ds_exp - kPExponent : 0.f);
+      nd_own[qq] = s[64];
+    }
+  }
+
   // ---- LDS operand addressing ----
   uint32_t row_rd[kKC];  // A operand of S and dP: row 16sb + c16, logical chunk 4c + g
 #pragma unroll
@@ -376,13 +389,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_bwd_kernel(BwdParams p)
     if (kKeys) acc2[db][0] = acc2[db][1] = f32x4{};
   }
 
-  auto decode = [&](int e_raw, int& st, int& flags) {
-    const int e = __builtin_amdgcn_readfirstlane(e_raw);
-    st = e >> 2;
-    flags = (st >= 0 && st < p.n_str_tiles) ? (e & 3) : 0;  // as in the forward
-    st = st < 0 ? 0 : (st < p.n_str_tiles ? st : p.n_str_tiles - 1);
-  };
-  auto entry = [&](int i) -> int { return kSparse ? list[i] : (((it0 + i) << 2) | 3); };
   auto tr_operand = [&](const unsigned char* a) -> V8 {
     const s16x4 lo = lds_read_tr16(a);
     const s16x4 hi = lds_read_tr16(a + 16 * L::kRowBytes);
@@ -473,11 +479,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_bwd_kernel(BwdParams p)
     }
   };
 
-  int st = 0, flags = 0;
-  if (n_iter > 0) {
-    decode(entry(0), st, flags);
-    dma(st, 0, 0);
-  }
   __builtin_amdgcn_s_waitcnt(0);  // V's DMA too, which must not outlive the workgroup
   __syncthreads();
   const int n_steps = n_iter * L::kSteps;
@@ -587,7 +588,7 @@ constexpr int kClasses = 6;
 
 __global__ __launch_bounds__(1024) void order_kernel(OrderParams p) {
   __shared__ int hist[kClasses][1024];
-  __shared__ long long total;
+  __shared__ float sums[16];
   __shared__ int start[kClasses];
   const int pass = blockIdx.x;
   const int n = p.tiles[pass];
@@ -597,15 +598,15 @@ __global__ __launch_bounds__(1024) void order_kernel(OrderParams p) {
   const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
   int sum = 0;
   for (int i = i0; i < i1; ++i) sum += counts[i];
-  hist[0][tid] = sum;
+  float part = static_cast<float>(sum);  // the mean only sets the classes' borders
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) part += __shfl_xor(part, m);
+  if (tid % 64 == 0) sums[tid / 64] = part;
   __syncthreads();
-  if (tid == 0) {
-    long long t = 0;
-    for (int i = 0; i < 1024; ++i) t += hist[0][i];
-    total = t;
-  }
-  __syncthreads();
-  const float mean = static_cast<float>(total) / n;
+  float mean = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) mean += sums[i];
+  mean /= n;
   auto class_of = [&](int c) {
     const float r = c / mean;
     return r >= 4.f ? 0 : r >= 2.8f ? 1 : r >= 2.f ? 2 : r >= 1.4f ? 3 : r >= 0.7f ? 4 : 5;

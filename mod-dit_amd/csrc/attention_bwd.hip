@@ -42,8 +42,12 @@ constexpr float kPExponent = 15.f;  // fp16: P is held as 2^15 P
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ s16x4 lds_read_tr16(const unsigned char* a) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a));
+// Reads at an LDS byte address.
+__device__ __forceinline__ s16x4 lds_read_tr16(uint32_t a) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4*>(a));
+}
+__device__ __forceinline__ u32x4 lds_read16(uint32_t a) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(a);
 }
 
 // At D = 128 the dK/dV pass has no registers for V beside its sums (128) and K (32): V stays in
@@ -68,6 +72,19 @@ struct BwdLds {
 template <int D>
 __device__ __forceinline__ int swz(int r) {
   return D == 128 ? 2 * (r & 7) + ((r >> 3) & 1) : 2 * ((r >> 1) & 3) + ((r >> 3) & 1);
+}
+
+// x, in registers from here on.
+template <typename V>
+__device__ __forceinline__ V pinned(V x) {
+  u32x4 u = __builtin_bit_cast(u32x4, x);
+  asm volatile("" : "+v"(u));
+  return __builtin_bit_cast(V, u);
+}
+template <>
+__device__ __forceinline__ uint32_t pinned(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 struct RowsOf {
@@ -232,8 +249,11 @@ __device__ __forceinline__ int ds_exponent(const float* maxima, int n, float (*r
   return e < -100 ? -100 : (e > 100 ? 100 : e);
 }
 
+// Waves per SIMD that the registers are held to.
+constexpr int bwd_waves(int head_dim) { return head_dim == 128 ? 2 : 3; }
+
 template <int D, typename E, bool kKeys, bool kSparse, bool kSplit>
-__global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void attention_bwd_kernel(BwdParams p) {
+__global__ __launch_bounds__(kThreads, bwd_waves(D)) __attribute__((amdgpu_waves_per_eu(bwd_waves(D), bwd_waves(D)))) void attention_bwd_kernel(BwdParams p) {
   using L = BwdLds<D, kKeys>;
   using V8 = typename E::vec8;
   constexpr int kKC = D / 32;  // MFMA k-steps over d
@@ -304,7 +324,6 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void attention_bwd_kern
       lds_dma16(rsrc2, dst + L::kTileBytes + (wave * L::kWinPerWave + i) * 1024, src2[i] + at * step2, 0);
     if (kKeys && wave == 0) lds_dma16(rsrc_st, dst + 2 * L::kTileBytes, lane * 16 + st * 512, 0);
   };
-  const unsigned char* const own2_lds = smem + 2 * L::kStage + wave * 32 * L::kRowBytes;
   if constexpr (L::kOwn2InLds) {
     const int64_t span = (static_cast<int64_t>(p.own_len) - 1) * p.own2.ss * 2 + L::kRowBytes;
     const u32x4 rsrc = raw_rsrc(p.own2.p + b * p.own2.sb + h * p.own2.sh, static_cast<uint32_t>(span));
@@ -332,13 +351,13 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void attention_bwd_kern
     dma(st, 0, 0);
   }
 
-  float ds_scale = 1.f;  // fp16, dK/dV: 2^(e - 15), from 2^15 P to 2^e dS
+  float ds_scale = 1.f;  // fp16: from P (dQ pass) or 2^15 P to 2^e dS
   float out1_scale = p.scale;
   int ds_exp = 0;
   if constexpr (kHalf) {
     __shared__ float red[4][4];
     ds_exp = ds_exponent(p.maxima + static_cast<int64_t>(bh) * p.n_maxima * 4, p.n_maxima, red);
-    ds_scale = ldexpf(1.f, ds_exp - static_cast<int>(kPExponent));
+    ds_scale = ldexpf(1.f, ds_exp - (kKeys ? static_cast<int>(kPExponent) : 0));
     out1_scale *= ldexpf(1.f, -ds_exp);
   }
 
@@ -363,7 +382,7 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void attention_bwd_kern
     for (int qq = 0; qq < 2; ++qq) {
       const int gr = ot * kBM + wave * 32 + 16 * qq + c16;
       const float* s = stats + (gr >> 6) * 128 + (gr & 63);
-      nl_own[qq] = s[0] + (kHalf ? ds_exp - kPExponent : 0.f);
+      nl_own[qq] = s[0] - (kHalf ? kPExponent : 0.f);
       nd_own[qq] = s[64];
     }
   }
@@ -372,15 +391,21 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void attention_bwd_kern
   uint32_t row_rd[kKC];  // A operand of S and dP: row 16sb + c16, logical chunk 4c + g
 #pragma unroll
   for (int c = 0; c < kKC; ++c)
-    row_rd[c] = static_cast<uint32_t>(c16 * L::kRowBytes + (((4 * c + g) ^ swz<D>(c16)) * 16));
+    row_rd[c] = pinned(static_cast<uint32_t>(lds0 + c16 * L::kRowBytes + (((4 * c + g) ^ swz<D>(c16)) * 16)));
   // A operand of the sums, transposed: see v_rd in attention.hip
   const int tr_row = 4 * g + (c16 >> 2);
   uint32_t tr_rd[kDB];
 #pragma unroll
   for (int db = 0; db < kDB; ++db) {
     const int d = db * 16 + 4 * (c16 & 3);
-    tr_rd[db] = static_cast<uint32_t>(tr_row * L::kRowBytes + (((d >> 3) ^ swz<D>(tr_row)) * 16) + (d & 7) * 2);
+    tr_rd[db] = pinned(static_cast<uint32_t>(lds0 + tr_row * L::kRowBytes + (((d >> 3) ^ swz<D>(tr_row)) * 16) + (d & 7) * 2));
   }
+
+  const uint32_t stats_rd = pinned(lds0 + 2 * L::kTileBytes + 16 * g);
+  uint32_t own2_rd[L::kOwn2InLds ? kKC : 1];
+  if constexpr (L::kOwn2InLds)
+#pragma unroll
+    for (int c = 0; c < kKC; ++c) own2_rd[c] = pinned(row_rd[c] + 2 * L::kStage + wave * 32 * L::kRowBytes);
 
   f32x4 acc1[kDB][2], acc2[kKeys ? kDB : 1][2];
 #pragma unroll
@@ -389,116 +414,186 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 3) void attention_bwd_kern
     if (kKeys) acc2[db][0] = acc2[db][1] = f32x4{};
   }
 
-  auto tr_operand = [&](const unsigned char* a) -> V8 {
+  auto tr_operand = [&](uint32_t a) -> V8 {
     const s16x4 lo = lds_read_tr16(a);
     const s16x4 hi = lds_read_tr16(a + 16 * L::kRowBytes);
     return as_vec8<V8>(u32x4{__builtin_bit_cast(u32x2, lo).x, __builtin_bit_cast(u32x2, lo).y,
                              __builtin_bit_cast(u32x2, hi).x, __builtin_bit_cast(u32x2, hi).y});
   };
 
-  // 32 streamed rows (half t of the tile) against the wave's 32 owned ones
-  auto half_tile = [&](const unsigned char* stage, int t, int st) {
-    const unsigned char* t1 = stage + (L::kSteps == 1 ? t * 32 * L::kRowBytes : 0);
-    const unsigned char* t2 = t1 + L::kTileBytes;
-    const float* stt = reinterpret_cast<const float*>(stage + 2 * L::kTileBytes);
+  // 32 streamed rows, from row `t0` of a stage on and with the statistics from `stat0` on (both
+  // known to the compiler, or nearly), against the wave's 32 owned ones
+  auto half_tile = [&](uint32_t t0, uint32_t stat0) {
     f32x4 s[2][2], dp[2][2], nl[2];
+    V8 pb[2], ds[2];
+    {  // S
 #pragma unroll
-    for (int sb = 0; sb < 2; ++sb) {
-      f32x4 nd;
-      if constexpr (kKeys) {
-        nl[sb] = *reinterpret_cast<const f32x4*>(stt + 32 * t + 16 * sb + 4 * g);
-        nd = *reinterpret_cast<const f32x4*>(stt + 64 + 32 * t + 16 * sb + 4 * g);
-      }
+      for (int sb = 0; sb < 2; ++sb) s[sb][0] = s[sb][1] = f32x4{};
 #pragma unroll
-      for (int qq = 0; qq < 2; ++qq) {
-        s[sb][qq] = f32x4{};
-        dp[sb][qq] = kKeys ? nd : f32x4{nd_own[qq], nd_own[qq], nd_own[qq], nd_own[qq]};
-      }
+      for (int c = 0; c < kKC; ++c)
+#pragma unroll
+        for (int sb = 0; sb < 2; ++sb) {
+          const V8 a = as_vec8<V8>(lds_read16(row_rd[c] + t0 + 16 * sb * L::kRowBytes));
+          s[sb][0] = E::mma16(a, own1[0][c], s[sb][0]);
+          s[sb][1] = E::mma16(a, own1[1][c], s[sb][1]);
+        }
     }
-#pragma unroll
-    for (int c = 0; c < kKC; ++c)
-#pragma unroll
-      for (int sb = 0; sb < 2; ++sb) {
-        const V8 a = *reinterpret_cast<const V8*>(t1 + row_rd[c] + 16 * sb * L::kRowBytes);
-        s[sb][0] = E::mma16(a, own1[0][c], s[sb][0]);
-        s[sb][1] = E::mma16(a, own1[1][c], s[sb][1]);
-      }
-#pragma unroll
-    for (int c = 0; c < kKC; ++c)
+    {  // dP - delta: the sums start from -delta
 #pragma unroll
       for (int sb = 0; sb < 2; ++sb) {
-        const V8 a = *reinterpret_cast<const V8*>(t2 + row_rd[c] + 16 * sb * L::kRowBytes);
-        if constexpr (L::kOwn2InLds) {
-#pragma unroll
-          for (int qq = 0; qq < 2; ++qq)
-            dp[sb][qq] = E::mma16(a, *reinterpret_cast<const V8*>(own2_lds + row_rd[c] + 16 * qq * L::kRowBytes), dp[sb][qq]);
+        if constexpr (kKeys) {
+          nl[sb] = __builtin_bit_cast(f32x4, lds_read16(stats_rd + stat0 + 64 * sb));
+          dp[sb][0] = dp[sb][1] = __builtin_bit_cast(f32x4, lds_read16(stats_rd + stat0 + 256 + 64 * sb));
         } else {
-          dp[sb][0] = E::mma16(a, own2[0][c], dp[sb][0]);
-          dp[sb][1] = E::mma16(a, own2[1][c], dp[sb][1]);
+#pragma unroll
+          for (int qq = 0; qq < 2; ++qq) dp[sb][qq] = f32x4{nd_own[qq], nd_own[qq], nd_own[qq], nd_own[qq]};
         }
       }
-    if constexpr (!kKeys) {
-      const int key0 = p.origin + st * kBN;
-      if (key0 < 0 || key0 + kBN > p.str_len) {
-        const int lo = -key0 - 32 * t - 4 * g, hi = p.str_len - key0 - 32 * t - 4 * g;
 #pragma unroll
-        for (int sb = 0; sb < 2; ++sb)
+      for (int c = 0; c < kKC; ++c) {
+        V8 o[2];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const bool out = 16 * sb + j < lo || 16 * sb + j >= hi;
-            s[sb][0][j] = out ? -INFINITY : s[sb][0][j];
-            s[sb][1][j] = out ? -INFINITY : s[sb][1][j];
-          }
+        for (int qq = 0; qq < 2; ++qq) {
+          if constexpr (L::kOwn2InLds)
+            o[qq] = as_vec8<V8>(lds_read16(own2_rd[c] + 16 * qq * L::kRowBytes));
+          else
+            o[qq] = own2[qq][c];
+        }
+#pragma unroll
+        for (int sb = 0; sb < 2; ++sb) {
+          const V8 a = as_vec8<V8>(lds_read16(row_rd[c] + t0 + L::kTileBytes + 16 * sb * L::kRowBytes));
+          dp[sb][0] = E::mma16(a, o[0], dp[sb][0]);
+          dp[sb][1] = E::mma16(a, o[1], dp[sb][1]);
+        }
       }
     }
-    V8 pb[2], db_[2];
-#pragma unroll
-    for (int qq = 0; qq < 2; ++qq)
+    {  // P into s; rounded to the storage type, the MFMA's operand
 #pragma unroll
       for (int sb = 0; sb < 2; ++sb)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float w = __builtin_amdgcn_exp2f(
-              __builtin_fmaf(s[sb][qq][j], p.scale_log2, kKeys ? nl[sb][j] : nl_own[qq]));
-          // rounded to the storage type, the MFMA's operand: 2^-9 (bf16) or 2^-12 (fp16) of each
-          // weight, the same as the forward's P
-          if (kKeys) pb[qq][4 * sb + j] = static_cast<typename E::elem>(w);
-          const float x = kHalf && kKeys ? w * ds_scale : w;
-          db_[qq][4 * sb + j] = static_cast<typename E::elem>(x * dp[sb][qq][j]);
-        }
+        for (int qq = 0; qq < 2; ++qq)
 #pragma unroll
-    for (int db = 0; db < kDB; ++db) {
-      const V8 a = tr_operand(t1 + tr_rd[db]);
-      acc1[db][0] = E::mma16(a, db_[0], acc1[db][0]);
-      acc1[db][1] = E::mma16(a, db_[1], acc1[db][1]);
-      if constexpr (kKeys) {
-        const V8 c = tr_operand(t2 + tr_rd[db]);
-        acc2[db][0] = E::mma16(c, pb[0], acc2[db][0]);
-        acc2[db][1] = E::mma16(c, pb[1], acc2[db][1]);
+          for (int j = 0; j < 4; ++j) {
+            const float arg = __builtin_fmaf(s[sb][qq][j], p.scale_log2, kKeys ? nl[sb][j] : nl_own[qq]);
+            float w = __builtin_amdgcn_exp2f(arg);
+            // P <= 1 but for rounding; keys outside the sequence (zeros, whose score is 0) may lie
+            // far above their row's LSE, and their weight times zero must stay zero
+            if (!kKeys) w = __builtin_amdgcn_fmed3f(w, 0.f, 1.f);
+            s[sb][qq][j] = w;
+            if (kKeys) pb[qq][4 * sb + j] = static_cast<typename E::elem>(w);
+          }
+    }
+    {  // dS
+#pragma unroll
+      for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+        for (int qq = 0; qq < 2; ++qq)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float x = kHalf ? s[sb][qq][j] * ds_scale : s[sb][qq][j];
+            ds[qq][4 * sb + j] = static_cast<typename E::elem>(x * dp[sb][qq][j]);
+          }
+    }
+    auto sums = [&](const V8 (&b)[2], f32x4 (&acc)[kDB][2], int off) {
+#pragma unroll
+      for (int db = 0; db < kDB; ++db) {
+        const V8 a = tr_operand(tr_rd[db] + t0 + off);
+        acc[db][0] = E::mma16(a, b[0], acc[db][0]);
+        acc[db][1] = E::mma16(a, b[1], acc[db][1]);
+      }
+    };
+    if constexpr (kKeys && D == 64) __builtin_amdgcn_sched_barrier(0);
+    if constexpr (kKeys) sums(pb, acc2, L::kTileBytes);
+    sums(ds, acc1, 0);
+
+    // Left to itself the compiler reads each operand right before its products and waits for it, and
+    // computes the weights with no product under way. In the dQ pass reads run kAhead operands ahead
+    // and the weights lie under the products of dP: 29,019 tokens x 12 heads, D = 128: 6.35 -> 5.79 ms;
+    // 17,776 x 16 block-sparse, D = 64: 0.80 -> 0.78 ms. The dK/dV pass at D = 64 gains by reads ahead of S
+    // and dP (1.15 -> 1.09 ms); at D = 128, where LDS reads take as long as the products, every order
+    // tried but the compiler's was 3 to 10 % slower.
+    constexpr int kAhead = 4;
+    constexpr int kRead = 0x100, kMma = 0x008, kValu = 0x002;
+    constexpr int n1 = 2 * kKC;  // operands of S, and of dP
+    if constexpr (!kKeys) {
+      constexpr int kExp = 32 / n1;
+      __builtin_amdgcn_sched_group_barrier(kRead, kAhead, 0);
+#pragma unroll
+      for (int i = 0; i < n1; ++i) {  // S
+        __builtin_amdgcn_sched_group_barrier(kMma, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(kRead, 1, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < n1 / 2; ++i) {  // dP and the weights
+        __builtin_amdgcn_sched_group_barrier(kMma, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(kRead, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kValu, kExp, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < n1 / 2; ++i) {  // reads reach into the sums' operands, two for each
+        __builtin_amdgcn_sched_group_barrier(kMma, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(kRead, 1 + kAhead * 2 / n1, 0);
+        __builtin_amdgcn_sched_group_barrier(kValu, kExp, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(kValu, 24, 0);  // dS
+#pragma unroll
+      for (int i = 0; i < kDB; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kMma, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(kRead, 2, 0);
+      }
+    } else if constexpr (D == 64) {
+      __builtin_amdgcn_sched_group_barrier(kRead, kAhead, 0);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kMma, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(kRead, 2, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < n1; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kMma, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(kRead, 1, 0);
       }
     }
   };
 
+  // the owned rows have arrived here: a wait for them inside the loop would wait for its DMA too
+#pragma unroll
+  for (int qq = 0; qq < 2; ++qq)
+#pragma unroll
+    for (int i = 0; i < kKC; ++i) {
+      own1[qq][i] = pinned(own1[qq][i]);
+      if constexpr (!L::kOwn2InLds) own2[qq][i] = pinned(own2[qq][i]);
+    }
   __builtin_amdgcn_s_waitcnt(0);  // V's DMA too, which must not outlive the workgroup
   __syncthreads();
   const int n_steps = n_iter * L::kSteps;
-  for (int j = 0; j < n_steps; ++j) {
+  // A step whose stage is known to the compiler: operand addresses are immediates of its reads.
+  auto step = [&](int j, auto stage_of_j) {
+    constexpr int kStageOff = decltype(stage_of_j)::value * L::kStage;
     const int part = j % L::kSteps;
     int st1 = st, flags1 = flags;
     if (j + 1 < n_steps) {
       if (part == L::kSteps - 1) decode(entry((j + 1) / L::kSteps), st1, flags1);
-      dma(st1, (j + 1) % L::kSteps, (j + 1) & 1);
+      dma(st1, (j + 1) % L::kSteps, 1 - decltype(stage_of_j)::value);
     }
     __builtin_amdgcn_sched_barrier(0);
-    const unsigned char* stage = smem + (j & 1) * L::kStage;
     if (flags & wbit) {
-      half_tile(stage, part, st);
-      if (L::kSteps == 1) half_tile(stage, 1, st);
+      if constexpr (L::kSteps == 1) {
+        half_tile(kStageOff, kStageOff);
+        __builtin_amdgcn_sched_barrier(0);
+        half_tile(kStageOff + 32 * L::kRowBytes, kStageOff + 128);
+      } else {
+        half_tile(kStageOff, kStageOff + 128 * part);
+      }
     }
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     st = st1;
     flags = flags1;
+  };
+  for (int j = 0; j < n_steps; j += 2) {
+    step(j, std::integral_constant<int, 0>{});
+    if (j + 1 < n_steps) step(j + 1, std::integral_constant<int, 1>{});
   }
 
   if constexpr (kSplit) {
@@ -796,7 +891,10 @@ struct BwdArgs {
   int64_t workspace_bytes;
 };
 
-RowsOf rows_of(const void* p, const int64_t* s) { return RowsOf{static_cast<const uint16_t*>(p), s[0], s[1], s[2]}; }
+// Rows of `len` tokens. A single row may come with any token stride.
+RowsOf rows_of(const void* p, const int64_t* s, int len, int dim) {
+  return RowsOf{static_cast<const uint16_t*>(p), s[0], s[1], len > 1 ? s[2] : dim};
+}
 
 int bwd_entry(const BwdArgs& a, moddit_stream_t stream) {
   clear_error();
@@ -845,21 +943,26 @@ int bwd_entry(const BwdArgs& a, moddit_stream_t stream) {
                    "attention_bwd: a 16-byte aligned workspace of %lld bytes is needed, got %lld",
                    static_cast<long long>(need), static_cast<long long>(a.workspace_bytes));
 
-  // Streamed rows are addressed with 32-bit byte offsets, a whole tile past the last included.
-  auto span = [](int len, const int64_t* s, int dim) { return len > 0 ? (static_cast<int64_t>(len) - 1) * s[2] * 2 + dim * 2 : 0; };
-  const int64_t spans[4] = {span(a.q_len, a.qs, a.head_dim), span(a.q_len, a.ds, a.head_dim),
-                            span(a.kv_len, a.ks, a.head_dim), span(a.kv_len, a.vs, a.head_dim)};
-  const int64_t last[4] = {nq * kBM * a.qs[2] * 2, nq * kBM * a.ds[2] * 2, nk * kBM * a.ks[2] * 2, nk * kBM * a.vs[2] * 2};
-  for (int i = 0; i < 4; ++i)
-    if (spans[i] > 0x7fffffffLL || last[i] > 0x7fffffffLL) {
+  const RowsOf q = rows_of(a.q, a.qs, a.q_len, a.head_dim), d = rows_of(a.d, a.ds, a.q_len, a.head_dim);
+  const RowsOf k = rows_of(a.k, a.ks, a.kv_len, a.head_dim), v = rows_of(a.v, a.vs, a.kv_len, a.head_dim);
+  // Streamed rows are addressed with 32-bit byte offsets, a whole tile past the last included; the
+  // rows past the last have to lie past the last's end, where they read as zeros.
+  const RowsOf streamed[4] = {q, d, k, v};
+  int64_t spans[4];
+  for (int i = 0; i < 4; ++i) {
+    const int64_t len = i < 2 ? a.q_len : a.kv_len, ss = streamed[i].ss;
+    MODDIT_CHECK_ARG(ss >= a.head_dim, "attention_bwd: token strides must be at least head_dim");
+    spans[i] = len > 0 ? (len - 1) * ss * 2 + a.head_dim * 2 : 0;
+    if (ss > (int64_t{1} << 31) || spans[i] > 0x7fffffffLL || (i < 2 ? nq : nk) * kBM * ss * 2 > 0x7fffffffLL) {
       set_error("attention_bwd: one head's rows exceed 2 GiB of 32-bit offsets");
       return MODDIT_EUNSUPPORTED;
     }
+  }
 
   StatsParams sp;
-  sp.o = rows_of(a.o, a.os);
-  sp.d = rows_of(a.d, a.ds);
-  sp.v = rows_of(a.v, a.vs);
+  sp.o = rows_of(a.o, a.os, a.q_len, a.head_dim);
+  sp.d = d;
+  sp.v = v;
   sp.lse = a.lse;
   sp.dlse = a.dlse;
   sp.heads = a.heads;
@@ -883,10 +986,10 @@ int bwd_entry(const BwdArgs& a, moddit_stream_t stream) {
   p.maxima = sp.maxima;
   p.n_maxima = sp.n_maxima;
   BwdParams dq = p, dkv = p;
-  dq.own1 = dkv.str1 = rows_of(a.q, a.qs);
-  dq.own2 = dkv.str2 = rows_of(a.d, a.ds);
-  dq.str1 = dkv.own1 = rows_of(a.k, a.ks);
-  dq.str2 = dkv.own2 = rows_of(a.v, a.vs);
+  dq.own1 = dkv.str1 = q;
+  dq.own2 = dkv.str2 = d;
+  dq.str1 = dkv.own1 = k;
+  dq.str2 = dkv.own2 = v;
   dq.out1 = static_cast<uint16_t*>(a.dq);
   dq.o1_sb = a.dqs[0]; dq.o1_sh = a.dqs[1]; dq.o1_ss = a.dqs[2];
   dq.out2 = nullptr;

@@ -287,7 +287,9 @@ def _attention_bwd(what, q, k, v, out, lse, grad_out, scale, grad_lse, tiles, ke
         _check_tiles(key_tiles, what)
         if key_tiles.counts.shape[0] != H or key_tiles.origin != origin or key_tiles.cap != 2 * tiles.n_qtiles:
             raise ValueError(f"{what}: key_tiles are not the transposed lists of tiles")
-    q, k, v, out, grad_out = (_attn_view(t) for t in (q, k, v, out, grad_out))
+    # rows of one token expanded along the sequence are stored out: the kernels tell rows by address
+    q, k, v, out, grad_out = (_attn_view(t if t.shape[2] < 2 or t.stride(2) >= D else t.contiguous())
+                              for t in (q, k, v, out, grad_out))
     lse, grad_lse = (None if t is None else t.contiguous() for t in (lse, grad_lse))
     dq, dk, dv = _empty_as(q), _empty_as(k), _empty_as(v)
     lib = _lib.load()

@@ -247,6 +247,9 @@ def test_broadcast_keys_and_unaligned_rows():
     q, k, v, do = _tensors(2, 3, 100, 150, 64, BF, False)
     e = lambda t: t[:1, :1].expand(2, 3, -1, -1)  # noqa: E731
     _run(q, e(k), e(v), do)
+    row = lambda t: t[:, :, :1].expand(-1, -1, 150, -1)  # noqa: E731
+    _run(q, row(k), row(v), do)  # one row for every token: past the last it must not be read
+    _run(row(q), k, v, row(do))
     odd = torch.randn((1, 2, 70, 65), generator=torch.Generator().manual_seed(1)).to(BF).cuda()[..., 1:]
     _run(odd, odd, odd, odd)
 

@@ -90,6 +90,7 @@ def _bwd(sparse=False, q=P, sizes=(1, 2, 64, 64, 64), stride=64, scale=0.125, dt
     (dict(ws=None), _lib.MODDIT_EINVAL, b"workspace"),
     (dict(ws=P + 4), _lib.MODDIT_EINVAL, b"workspace"),
     (dict(nbytes=16), _lib.MODDIT_EINVAL, b"workspace"),
+    (dict(stride=0), _lib.MODDIT_EINVAL, b"at least head_dim"),
     (dict(stride=1 << 25), _lib.MODDIT_EUNSUPPORTED, b"2 GiB"),
     (dict(sparse=True, lists=(None, P, 1, 1, P, P, 1, 2)), _lib.MODDIT_EINVAL, b"counts"),
     (dict(sparse=True, lists=(P, P, 1, 1, None, P, 1, 2)), _lib.MODDIT_EINVAL, b"lists missing"),

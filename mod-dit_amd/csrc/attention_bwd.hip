@@ -7,7 +7,7 @@
 // A (row, key) pair takes 10 D FLOP. P is computed again from Q, K and the LSE: nothing of the
 // size of P is kept.
 //
-// Two passes of one kernel body. Each workgroup owns 128 rows of one side and streams tiles of 64
+// Two passes of one kernel body, in one launch. Each workgroup owns 128 rows of one side and streams tiles of 64
 // rows of the other: the dQ pass owns queries and streams keys, the dK/dV pass owns keys and
 // streams queries, so every sum stays in one workgroup's registers: no atomics, and results do
 // not depend on the order of workgroups. The price is that S and dP are computed twice, 14 D FLOP
@@ -119,6 +119,7 @@ struct BwdParams {
   // part [tile][piece][dQ, or dK and dV][128][D]
   int n_split;
   float* part;
+  int n_groups;  // workgroups of the pass
 };
 
 // ---- row statistics ----
@@ -249,11 +250,9 @@ __device__ __forceinline__ int ds_exponent(const float* maxima, int n, float (*r
   return e < -100 ? -100 : (e > 100 ? 100 : e);
 }
 
-// Waves per SIMD that the registers are held to.
-constexpr int bwd_waves(int head_dim) { return head_dim == 128 ? 2 : 3; }
-
-template <int D, typename E, bool kKeys, bool kSparse, bool kSplit>
-__global__ __launch_bounds__(kThreads, bwd_waves(D)) __attribute__((amdgpu_waves_per_eu(bwd_waves(D), bwd_waves(D)))) void attention_bwd_kernel(BwdParams p) {
+// Workgroup `wg` of one pass.
+template <int D, typename E, bool kKeys, bool kSparse>
+__device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) {
   using L = BwdLds<D, kKeys>;
   using V8 = typename E::vec8;
   constexpr int kKC = D / 32;  // MFMA k-steps over d
@@ -267,8 +266,9 @@ __global__ __launch_bounds__(kThreads, bwd_waves(D)) __attribute__((amdgpu_waves
   const int g = lane >> 4;
   const int c16 = lane & 15;
 
-  int tile = kSplit ? blockIdx.x / p.n_split : xcd_remap(blockIdx.x, gridDim.x, p.xcd_run);
-  if (kSparse && !kSplit && p.order != nullptr) tile = p.order[tile];
+  const bool split = p.n_split > 1;
+  int tile = split ? wg / p.n_split : xcd_remap(wg, p.n_groups, p.xcd_run);
+  if (kSparse && !split && p.order != nullptr) tile = p.order[tile];
   const int ot = tile % p.n_tiles;
   const int bh = tile / p.n_tiles;
   const int b = bh / p.heads;
@@ -283,8 +283,8 @@ __global__ __launch_bounds__(kThreads, bwd_waves(D)) __attribute__((amdgpu_waves
     list = p.entries + slot * p.cap;
   }
   int it0 = 0;  // first streamed tile (dense) of this workgroup's piece
-  if constexpr (kSplit) {
-    const int piece = blockIdx.x - tile * p.n_split;
+  if (split) {
+    const int piece = wg - tile * p.n_split;
     const int first = static_cast<int>(static_cast<int64_t>(n_iter) * piece / p.n_split);
     n_iter = static_cast<int>(static_cast<int64_t>(n_iter) * (piece + 1) / p.n_split) - first;
     if (kSparse)
@@ -596,8 +596,8 @@ __global__ __launch_bounds__(kThreads, bwd_waves(D)) __attribute__((amdgpu_waves
     if (j + 1 < n_steps) step(j + 1, std::integral_constant<int, 1>{});
   }
 
-  if constexpr (kSplit) {
-    float* part = p.part + static_cast<int64_t>(blockIdx.x) * (kKeys ? 2 : 1) * kBM * D;
+  if (split) {
+    float* part = p.part + static_cast<int64_t>(wg) * (kKeys ? 2 : 1) * kBM * D;
 #pragma unroll
     for (int qq = 0; qq < 2; ++qq) {
       float* r = part + (wave * 32 + 16 * qq + c16) * D + 4 * g;
@@ -636,18 +636,43 @@ __global__ __launch_bounds__(kThreads, bwd_waves(D)) __attribute__((amdgpu_waves
   }
 }
 
+// Waves per SIMD that the registers are held to.
+constexpr int bwd_waves(int head_dim) { return head_dim == 128 ? 2 : 3; }
+
+// Both passes in one launch: they need nothing of each other, and the end of the one is filled by
+// the other. The one whose workgroups take longer comes first; the other starts at a multiple of the
+// XCDs so that both keep their order of tiles.
+struct BothPasses {
+  BwdParams dkv, dq;
+  int first_dkv, first_dq;
+};
+
+template <int D, typename E, bool kSparse>
+__global__ __launch_bounds__(kThreads, bwd_waves(D)) __attribute__((amdgpu_waves_per_eu(bwd_waves(D), bwd_waves(D)))) void attention_bwd_kernel(BothPasses p) {
+  const int keys = static_cast<int>(blockIdx.x) - p.first_dkv, rows = static_cast<int>(blockIdx.x) - p.first_dq;
+  if (keys >= 0 && keys < p.dkv.n_groups)
+    bwd_workgroup<D, E, true, kSparse>(p.dkv, keys);
+  else if (rows >= 0 && rows < p.dq.n_groups)
+    bwd_workgroup<D, E, false, kSparse>(p.dq, rows);
+}
+
 // The pieces of a tile -> its rows, added in piece order. A workgroup takes kCombineRows rows of
 // one tile and tensor, a thread four of its columns. Bound by reading the partials back, mostly
 // from L2 and the last-level cache.
 constexpr int kCombineRows = 16;
 
-template <int D, typename E, bool kKeys>
-__global__ __launch_bounds__(kThreads) void combine_bwd_kernel(BwdParams p) {
+template <int D, typename E>
+__global__ __launch_bounds__(kThreads) void combine_bwd_kernel(BothPasses both, int first_dq) {
   constexpr int kCols = D / 4;
-  constexpr int kTensors = kKeys ? 2 : 1;
-  const int tile = blockIdx.x / (kBM / kCombineRows);
-  const int r_first = (blockIdx.x % (kBM / kCombineRows)) * kCombineRows;
-  const bool second = kKeys && blockIdx.y == 1;
+  constexpr int kParts = kBM / kCombineRows;
+  const bool keys = static_cast<int>(blockIdx.x) < first_dq;
+  const BwdParams& p = keys ? both.dkv : both.dq;
+  const int tensors = keys ? 2 : 1;
+  int i0 = keys ? blockIdx.x : blockIdx.x - first_dq;
+  const int r_first = (i0 % kParts) * kCombineRows;
+  i0 /= kParts;
+  const int second = i0 % tensors;
+  const int tile = i0 / tensors;
   const int ot = tile % p.n_tiles;
   const int bh = tile / p.n_tiles;
   const int b = bh / p.heads, h = bh % p.heads;
@@ -655,9 +680,9 @@ __global__ __launch_bounds__(kThreads) void combine_bwd_kernel(BwdParams p) {
   for (int r = r_first + threadIdx.x / kCols; r < r_first + kCombineRows; r += kThreads / kCols) {
     const int row = p.origin + ot * kBM + r;
     if (row < 0 || row >= p.own_len) continue;
-    const float* at = p.part + ((static_cast<int64_t>(tile) * p.n_split * kTensors + second) * kBM + r) * D + d;
+    const float* at = p.part + ((static_cast<int64_t>(tile) * p.n_split * tensors + second) * kBM + r) * D + d;
     f32x4 x = f32x4{};
-    for (int i = 0; i < p.n_split; ++i) x += *reinterpret_cast<const f32x4*>(at + static_cast<int64_t>(i) * kTensors * kBM * D);
+    for (int i = 0; i < p.n_split; ++i) x += *reinterpret_cast<const f32x4*>(at + static_cast<int64_t>(i) * tensors * kBM * D);
     u32x2 w;
     w.x = pack2(E::from_float(x[0]), E::from_float(x[1]));
     w.y = pack2(E::from_float(x[2]), E::from_float(x[3]));
@@ -753,38 +778,30 @@ __global__ __launch_bounds__(1024) void order_kernel(OrderParams p) {
   }
 }
 
-template <int D, typename E, bool kKeys, bool kSparse, bool kSplit>
-int launch_pass(const BwdParams& p, int batch, hipStream_t st) {
-  constexpr int kLds = BwdLds<D, kKeys>::kTotal;
-  auto kernel = attention_bwd_kernel<D, E, kKeys, kSparse, kSplit>;
+template <int D, typename E, bool kSparse>
+int launch_passes(const BothPasses& p, hipStream_t st) {
+  constexpr int kLds = BwdLds<D, true>::kTotal > BwdLds<D, false>::kTotal ? BwdLds<D, true>::kTotal : BwdLds<D, false>::kTotal;
+  auto kernel = attention_bwd_kernel<D, E, kSparse>;
   static LaunchSetup once;
   if (set_dynamic_lds_once(once, reinterpret_cast<const void*>(kernel), kLds) != hipSuccess) {
     set_error("attention_bwd: cannot reserve %d bytes of LDS", kLds);
     return MODDIT_EHIP;
   }
-  const int64_t tiles = static_cast<int64_t>(batch) * p.heads * p.n_tiles;
-  if (tiles == 0) return MODDIT_OK;
-  const int64_t grid = kSplit ? tiles * p.n_split : tiles;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), kLds, st, p);
+  const int last_dq = p.first_dq + p.dq.n_groups, last_dkv = p.first_dkv + p.dkv.n_groups;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(last_dq > last_dkv ? last_dq : last_dkv)), dim3(kThreads), kLds, st, p);
   MODDIT_CHECK_LAUNCH("attention_bwd");
-  if constexpr (kSplit) {
-    hipLaunchKernelGGL((combine_bwd_kernel<D, E, kKeys>), dim3(static_cast<unsigned>(tiles * (kBM / kCombineRows)), kKeys ? 2 : 1),
-                       dim3(kThreads), 0, st, p);
+  auto combined = [](const BwdParams& q) { return q.n_split > 1 ? q.n_groups / q.n_split * (kBM / kCombineRows) : 0; };
+  const int first_dq = 2 * combined(p.dkv), groups = first_dq + combined(p.dq);
+  if (groups > 0) {
+    hipLaunchKernelGGL((combine_bwd_kernel<D, E>), dim3(groups), dim3(kThreads), 0, st, p, first_dq);
     MODDIT_CHECK_LAUNCH("attention_bwd (combine)");
   }
   return MODDIT_OK;
 }
 
-template <int D, typename E, bool kKeys>
-int launch_side(const BwdParams& p, int batch, hipStream_t st) {
-  const bool sparse = p.counts != nullptr;
-  if (p.n_split > 1)
-    return sparse ? launch_pass<D, E, kKeys, true, true>(p, batch, st) : launch_pass<D, E, kKeys, false, true>(p, batch, st);
-  return sparse ? launch_pass<D, E, kKeys, true, false>(p, batch, st) : launch_pass<D, E, kKeys, false, false>(p, batch, st);
-}
-
 template <int D, typename E>
-int launch_bwd(const StatsParams& sp, const BwdParams& dq, const BwdParams& dkv, int batch, hipStream_t st) {
+int launch_bwd(const StatsParams& sp, const BothPasses& p, int batch, hipStream_t st) {
+  const BwdParams &dq = p.dq, &dkv = p.dkv;
   constexpr bool kMax = std::is_same<E, Fp16>::value;
   const int blocks = kMax ? sp.n_maxima : sp.stat_blocks;
   if (blocks > 0) {
@@ -797,8 +814,7 @@ int launch_bwd(const StatsParams& sp, const BwdParams& dq, const BwdParams& dkv,
     hipLaunchKernelGGL(order_kernel, dim3(2), dim3(1024), 0, st, op);
     MODDIT_CHECK_LAUNCH("attention_bwd (order)");
   }
-  if (const int rc = launch_side<D, E, false>(dq, batch, st)) return rc;
-  return launch_side<D, E, true>(dkv, batch, st);
+  return dq.counts != nullptr ? launch_passes<D, E, true>(p, st) : launch_passes<D, E, false>(p, st);
 }
 
 // ---- sizes ----
@@ -809,40 +825,18 @@ int64_t maxima_of(int q_len, int kv_len, int origin) {
   return a > b ? a : b;
 }
 
-// How many workgroups share a tile's streamed range: see split_for in attention.hip; here the
-// partial sums are dQ's, or dK's and dV's.
+// Microseconds of a streamed tile of 64 rows in a workgroup of the dQ or dK/dV pass while the card
+// is full, and the workgroups that fill it.
+double step_us(int head_dim, bool keys) { return head_dim == 128 ? (keys ? 3.4 : 2.3) : (keys ? 3.0 : 2.3); }
+int resident(int head_dim) { return head_dim == 128 ? 512 : 768; }
+constexpr int kFixedSteps = 4;  // a workgroup's start and end, in steps
 constexpr int kMaxSplit = 64;
-
-double cu_step_us(int head_dim, bool keys, int64_t k) {
-  constexpr double t128[2][2] = {{1.63, 2.6}, {2.3, 3.64}}, t64[2][3] = {{0.9, 1.2, 1.6}, {1.2, 1.6, 2.2}};
-  if (head_dim == 128) return k <= 2 ? t128[keys][k - 1] : t128[keys][1] / 2 * k;
-  return k <= 3 ? t64[keys][k - 1] : t64[keys][2] / 3 * k;
-}
-
-int split_for(int64_t tiles, int64_t steps, int head_dim, bool keys) {
-  constexpr double kCus = 256, kFixedSteps = 4, kLaunchUs = 5.0, kPartialBytesPerUs = 4.0e6;
-  int best = 1;
-  double best_us = 0.0;
-  if (tiles == 0) return 1;
-  for (int s = 1; s <= kMaxSplit; ++s) {
-    if (s > 1 && steps < 4 * static_cast<int64_t>(s)) break;
-    const int64_t per_cu = static_cast<int64_t>((tiles * s + kCus - 1) / kCus);
-    double us = cu_step_us(head_dim, keys, per_cu) * (static_cast<double>(steps) / s + kFixedSteps);
-    if (s > 1) us += kLaunchUs + tiles * s * (kBM * head_dim * 8.0 * (keys ? 2 : 1)) / kPartialBytesPerUs;
-    if (s == 1 || us < 0.97 * best_us) {
-      best = s;
-      best_us = us;
-    }
-  }
-  return best;
-}
-
-constexpr int64_t kResident = 512;  // workgroups that run at once at least: fewer tiles need no order
+constexpr int kMinPiece = 4;  // steps of a piece at the least
 
 struct BwdPlan {
   int64_t stat_blocks, n_maxima, tiles[2];
   int n_split[2];
-  bool order;
+  bool order, dq_first;
   int64_t stats, maxima, orders, parts[2], total;  // floats, each from a multiple of 4
 };
 
@@ -858,8 +852,28 @@ BwdPlan plan_bwd(int batch, int heads, int q_len, int kv_len, int head_dim, int 
   p.tiles[0] = tiles_of(q_len);
   p.tiles[1] = tiles_of(kv_len);
   const int64_t steps[2] = {cap > 0 ? cap / 4 : steps_of(kv_len), key_cap > 0 ? key_cap / 4 : steps_of(q_len)};
-  for (int i = 0; i < 2; ++i) p.n_split[i] = split_for(bh * p.tiles[i], steps[i], head_dim, i == 1);
-  p.order = cap > 0 && bh * (p.tiles[0] > p.tiles[1] ? p.tiles[0] : p.tiles[1]) > kResident;
+  // A launch lasts as long as all its steps on a full card, or as its longest workgroup. Where few
+  // tiles sweep long ranges (a text tail, a short clip, few heads) the sweep of a tile is shared among
+  // workgroups, so that none takes longer than the whole on a full card, at the price of writing and
+  // adding fp32 partial sums and one more launch (5 us). 256 rows x 29,019 keys x 24 heads, D = 128:
+  // 1,240 us without, 440 with; 4,096 tokens x 2 heads, D = 64: 178 and 73.
+  double all_us = 0.0, piece_us[2];
+  for (int i = 0; i < 2; ++i) all_us += bh * p.tiles[i] * (steps[i] + kFixedSteps) * step_us(head_dim, i == 1);
+  all_us /= resident(head_dim);
+  for (int i = 0; i < 2; ++i) {
+    const double sweep_us = steps[i] * step_us(head_dim, i == 1);
+    int64_t n = 1;
+    if (sweep_us > all_us + 10.0) {
+      n = static_cast<int64_t>(std::ceil(sweep_us / all_us));
+      if (n > kMaxSplit) n = kMaxSplit;
+      if (n > steps[i] / kMinPiece) n = steps[i] / kMinPiece;
+      if (n < 1) n = 1;
+    }
+    p.n_split[i] = static_cast<int>(n);
+    piece_us[i] = sweep_us / n;
+  }
+  p.dq_first = piece_us[0] > piece_us[1];
+  p.order = cap > 0 && bh * (p.tiles[0] + p.tiles[1]) > resident(head_dim);
   auto up4 = [](int64_t x) { return (x + 3) / 4 * 4; };
   p.stats = 0;
   p.maxima = p.stats + bh * p.stat_blocks * 128;
@@ -867,10 +881,9 @@ BwdPlan plan_bwd(int batch, int heads, int q_len, int kv_len, int head_dim, int 
   int64_t at = p.orders + (p.order ? up4(bh * (p.tiles[0] + p.tiles[1])) : 0);
   for (int i = 0; i < 2; ++i) {
     p.parts[i] = at;
-    // the passes run one after the other, each with its combine: they share the room
-    const int64_t n = p.n_split[i] > 1 ? bh * p.tiles[i] * p.n_split[i] * kBM * head_dim * (i + 1) : 0;
-    p.total = i == 0 ? at + n : (at + n > p.total ? at + n : p.total);
+    if (p.n_split[i] > 1) at += bh * p.tiles[i] * p.n_split[i] * kBM * head_dim * (i + 1);
   }
+  p.total = at;
   return p;
 }
 
@@ -937,8 +950,7 @@ int bwd_entry(const BwdArgs& a, moddit_stream_t stream) {
                                 lists ? a.key_cap : 0);
   const int64_t need = plan.total * 4;
   for (int i = 0; i < 2; ++i)
-    MODDIT_CHECK_ARG(plan.tiles[i] * a.batch * a.heads * (kBM / kCombineRows) * plan.n_split[i] <= 0x7fffffff,
-                     "attention_bwd: too many tiles");
+    MODDIT_CHECK_ARG(plan.tiles[i] * a.batch * a.heads * plan.n_split[i] <= 0x7ffffff, "attention_bwd: too many tiles");
   MODDIT_CHECK_ARG((a.workspace != nullptr || need == 0) && aligned16(a.workspace) && a.workspace_bytes >= need,
                    "attention_bwd: a 16-byte aligned workspace of %lld bytes is needed, got %lld",
                    static_cast<long long>(need), static_cast<long long>(a.workspace_bytes));
@@ -1028,11 +1040,15 @@ int bwd_entry(const BwdArgs& a, moddit_stream_t stream) {
     dq.xcd_run = dkv.xcd_run = kXcdRun;
   }
 
+  dq.n_groups = static_cast<int>(plan.tiles[0] * a.batch * a.heads * plan.n_split[0]);
+  dkv.n_groups = static_cast<int>(plan.tiles[1] * a.batch * a.heads * plan.n_split[1]);
+  const int first = ((plan.dq_first ? dq : dkv).n_groups + kNumXcd - 1) / kNumXcd * kNumXcd;
+  const BothPasses both{dkv, dq, plan.dq_first ? first : 0, plan.dq_first ? 0 : first};
   hipStream_t st = as_stream(stream);
   const bool bf = a.dtype == MODDIT_BF16;
   if (a.head_dim == 128)
-    return bf ? launch_bwd<128, Bf16>(sp, dq, dkv, a.batch, st) : launch_bwd<128, Fp16>(sp, dq, dkv, a.batch, st);
-  return bf ? launch_bwd<64, Bf16>(sp, dq, dkv, a.batch, st) : launch_bwd<64, Fp16>(sp, dq, dkv, a.batch, st);
+    return bf ? launch_bwd<128, Bf16>(sp, both, a.batch, st) : launch_bwd<128, Fp16>(sp, both, a.batch, st);
+  return bf ? launch_bwd<64, Bf16>(sp, both, a.batch, st) : launch_bwd<64, Fp16>(sp, both, a.batch, st);
 }
 
 // ---- tile lists by key tile ----

@@ -39,6 +39,7 @@ constexpr int kBN = 64;   // streamed rows per tile
 constexpr int kThreads = 256;
 constexpr int kStatsBytes = 1024;  // one DMA window; a block's 64 -LSE and 64 -delta take half
 constexpr float kPExponent = 15.f;  // fp16: P is held as 2^15 P
+constexpr int kFewKeys = 64;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
@@ -135,11 +136,18 @@ struct StatsParams {
   int stat_blocks;
   int n_maxima;
   float p_exponent;
+  int one_key;         // kv_len == 1, see below
+  uint16_t* zero_row;  // then: D zeros to write
+  RowsOf q, k;         // few_keys_kernel
+  float scale_log2;
 };
 
 // Block i of a head: -LSE (log2 units, with the exponent that P is held at) and -delta of the 64
 // grid rows from 64 i on; with kMax also the largest finite |dO|^2, |O|^2, |V|^2 and |dL| of its rows.
 // Reads O, dO (and V) once: bound by HBM.
+//
+// The softmax over one key is 1 whatever its score: dP = delta, and dS = P dL exactly. The rounding of
+// O and of the sums would leave a remainder, so delta keeps -dL alone there and the passes see a zero V.
 template <int D, typename E, bool kMax>
 __global__ __launch_bounds__(kThreads) void stats_kernel(StatsParams p) {
   constexpr int kLanes = D / 8;
@@ -152,6 +160,8 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(StatsParams p) {
   float top[4] = {0.f, 0.f, 0.f, 0.f};
   // a row that is not finite spoils what it reaches whatever the scale, and must not set the others'
   auto finite_max = [](float m, float x) { return x < INFINITY ? fmaxf(m, x) : m; };
+  if (p.one_key && blk == 0 && bh == 0 && threadIdx.x < kLanes)
+    reinterpret_cast<u32x4*>(p.zero_row)[threadIdx.x] = u32x4{0, 0, 0, 0};
   auto row_sum = [](float x) {
 #pragma unroll
     for (int m = 1; m < kLanes; m *= 2) x += __shfl_xor(x, m);
@@ -194,7 +204,7 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(StatsParams p) {
       if (l == 0) {
         float* s = p.stats + (static_cast<int64_t>(bh) * p.stat_blocks + blk) * 128;
         s[r] = nl;
-        s[64 + r] = in ? g - dot : 0.f;
+        s[64 + r] = in ? (p.one_key ? g : g - dot) : 0.f;
       }
     }
     if (kMax) {
@@ -221,6 +231,70 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(StatsParams p) {
     if (threadIdx.x < 4)
       p.maxima[(static_cast<int64_t>(bh) * p.n_maxima + blk) * 4 + threadIdx.x] =
           fmaxf(fmaxf(red[0][threadIdx.x], red[1][threadIdx.x]), fmaxf(red[2][threadIdx.x], red[3][threadIdx.x]));
+  }
+}
+
+// The same for bf16 and at most 64 keys, with delta = sum_j P_ij dP_ij / sum_j P_ij in place of
+// dO O: over few keys O is as large as V, and its rounding (2^-8 of it) in delta exceeds that of dS
+// (two keys, D = 64: dQ 5.2e-3 off its 64-bit value in place of 2.4e-3). One wave per 32 rows; the keys'
+// rows come from global memory as the products' operands, shared by all workgroups of a head.
+template <int D, typename E>
+__global__ __launch_bounds__(kThreads) void few_keys_kernel(StatsParams p) {
+  using V8 = typename E::vec8;
+  constexpr int kKC = D / 32;
+  const int bh = blockIdx.y;
+  const int b = bh / p.heads, h = bh % p.heads;
+  const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
+  const int row0 = blockIdx.x * kBM + (threadIdx.x >> 6) * 32 + c16;
+  auto operand = [&](const RowsOf& t, int row, int c) {
+    return as_vec8<V8>(reinterpret_cast<const u32x4*>(t.p + b * t.sb + h * t.sh + row * t.ss)[4 * c + g]);
+  };
+  V8 q[2][kKC], d[2][kKC];
+  float nl[2], gl[2], num[2] = {0.f, 0.f}, den[2] = {0.f, 0.f};
+#pragma unroll
+  for (int qq = 0; qq < 2; ++qq) {
+    const int row = row0 + 16 * qq < p.q_len ? row0 + 16 * qq : p.q_len - 1;
+    const int64_t at = static_cast<int64_t>(bh) * p.q_len + row;
+    const float lse = p.lse[at];
+    nl[qq] = lse == -INFINITY ? -INFINITY : -lse * 1.4426950408889634f;
+    gl[qq] = p.dlse != nullptr ? p.dlse[at] : 0.f;
+#pragma unroll
+    for (int c = 0; c < kKC; ++c) {
+      q[qq][c] = operand(p.q, row, c);
+      d[qq][c] = operand(p.d, row, c);
+    }
+  }
+  for (int key0 = 0; key0 < p.kv_len; key0 += 16) {
+    const int key = key0 + c16 < p.kv_len ? key0 + c16 : p.kv_len - 1;
+    f32x4 s[2] = {f32x4{}, f32x4{}}, dp[2] = {f32x4{}, f32x4{}};
+#pragma unroll
+    for (int c = 0; c < kKC; ++c) {
+      const V8 k = operand(p.k, key, c), v = operand(p.v, key, c);
+#pragma unroll
+      for (int qq = 0; qq < 2; ++qq) {
+        s[qq] = E::mma16(k, q[qq][c], s[qq]);
+        dp[qq] = E::mma16(v, d[qq][c], dp[qq]);
+      }
+    }
+#pragma unroll
+    for (int qq = 0; qq < 2; ++qq)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (key0 + 4 * g + j >= p.kv_len) continue;
+        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qq][j], p.scale_log2, nl[qq]));
+        num[qq] += w * dp[qq][j];
+        den[qq] += w;
+      }
+  }
+#pragma unroll
+  for (int qq = 0; qq < 2; ++qq) {
+    const float n = sum_over_groups(num[qq]), m = sum_over_groups(den[qq]);
+    const int row = row0 + 16 * qq;
+    if (g == 0) {
+      float* s = p.stats + (static_cast<int64_t>(bh) * p.stat_blocks + (row >> 6)) * 128 + (row & 63);
+      s[0] = row < p.q_len ? nl[qq] : -INFINITY;
+      s[64] = row < p.q_len ? gl[qq] - (m != 0.f ? n / m : 0.f) : 0.f;
+    }
   }
 }
 
@@ -804,7 +878,15 @@ int launch_bwd(const StatsParams& sp, const BothPasses& p, int batch, hipStream_
   const BwdParams &dq = p.dq, &dkv = p.dkv;
   constexpr bool kMax = std::is_same<E, Fp16>::value;
   const int blocks = kMax ? sp.n_maxima : sp.stat_blocks;
-  if (blocks > 0) {
+  bool done = false;
+  if constexpr (!kMax) {
+    if (dq.counts == nullptr && sp.kv_len > 1 && sp.kv_len <= kFewKeys && sp.q_len > 0) {
+      hipLaunchKernelGGL((few_keys_kernel<D, E>), dim3(dq.n_tiles, batch * sp.heads), dim3(kThreads), 0, st, sp);
+      MODDIT_CHECK_LAUNCH("attention_bwd (few keys)");
+      done = true;
+    }
+  }
+  if (!done && blocks > 0) {
     hipLaunchKernelGGL((stats_kernel<D, E, kMax>), dim3(blocks, batch * sp.heads), dim3(kThreads), 0, st, sp);
     MODDIT_CHECK_LAUNCH("attention_bwd (row statistics)");
   }
@@ -837,7 +919,7 @@ struct BwdPlan {
   int64_t stat_blocks, n_maxima, tiles[2];
   int n_split[2];
   bool order, dq_first;
-  int64_t stats, maxima, orders, parts[2], total;  // floats, each from a multiple of 4
+  int64_t stats, zero_row, maxima, orders, parts[2], total;  // floats, each from a multiple of 4
 };
 
 // What a call of these sizes runs and keeps in its workspace. cap, key_cap: 0 for dense calls; a
@@ -876,7 +958,8 @@ BwdPlan plan_bwd(int batch, int heads, int q_len, int kv_len, int head_dim, int 
   p.order = cap > 0 && bh * (p.tiles[0] + p.tiles[1]) > resident(head_dim);
   auto up4 = [](int64_t x) { return (x + 3) / 4 * 4; };
   p.stats = 0;
-  p.maxima = p.stats + bh * p.stat_blocks * 128;
+  p.zero_row = p.stats + bh * p.stat_blocks * 128;
+  p.maxima = p.zero_row + (kv_len == 1 ? head_dim / 2 : 0);
   p.orders = p.maxima + bh * p.n_maxima * 4;
   int64_t at = p.orders + (p.order ? up4(bh * (p.tiles[0] + p.tiles[1])) : 0);
   for (int i = 0; i < 2; ++i) {
@@ -987,6 +1070,11 @@ int bwd_entry(const BwdArgs& a, moddit_stream_t stream) {
   sp.stats = ws + plan.stats;
   sp.maxima = ws + plan.maxima;
   sp.p_exponent = a.dtype == MODDIT_FP16 ? kPExponent : 0.f;
+  sp.one_key = a.kv_len == 1;
+  sp.zero_row = reinterpret_cast<uint16_t*>(ws + plan.zero_row);
+  sp.q = q;
+  sp.k = k;
+  sp.scale_log2 = a.scale * 1.4426950408889634f;
 
   BwdParams p;
   p.heads = a.heads;
@@ -1001,7 +1089,7 @@ int bwd_entry(const BwdArgs& a, moddit_stream_t stream) {
   dq.own1 = dkv.str1 = q;
   dq.own2 = dkv.str2 = d;
   dq.str1 = dkv.own1 = k;
-  dq.str2 = dkv.own2 = v;
+  dq.str2 = dkv.own2 = a.kv_len == 1 ? RowsOf{sp.zero_row, 0, 0, a.head_dim} : v;
   dq.out1 = static_cast<uint16_t*>(a.dq);
   dq.o1_sb = a.dqs[0]; dq.o1_sh = a.dqs[1]; dq.o1_ss = a.dqs[2];
   dq.out2 = nullptr;
@@ -1026,7 +1114,7 @@ int bwd_entry(const BwdArgs& a, moddit_stream_t stream) {
   dkv.str1_bytes = static_cast<uint32_t>(spans[0]);
   dkv.str2_bytes = static_cast<uint32_t>(spans[1]);
   dq.str1_bytes = static_cast<uint32_t>(spans[2]);
-  dq.str2_bytes = static_cast<uint32_t>(spans[3]);
+  dq.str2_bytes = static_cast<uint32_t>(a.kv_len == 1 ? a.head_dim * 2 : spans[3]);
   dq.counts = lists ? a.counts : nullptr;
   dq.entries = a.entries;
   dq.cap = a.cap;

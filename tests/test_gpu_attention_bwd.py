@@ -31,9 +31,10 @@ def _tensors(B, H, Sq, Skv, D, dtype, nhd, seed=0, qscale=1.0, gscale=1.0):
     return one(Sq, qscale), one(Skv), one(Skv), one(Sq, gscale)
 
 
-def _ref(q, k, v, do, scale, mask=None, dlse=None):
+def _ref(q, k, v, do, scale, mask=None, dlse=None, u_out=None):
     """out, lse, gradients in 64 bits, and the gradients' tolerances (u |x| aside)."""
     u = torch.finfo(q.dtype).eps / 2
+    u_out = u if u_out is None else u_out
     q, k, v, do = (t.double() for t in (q, k, v, do))
     s = q @ k.transpose(2, 3) * scale
     if mask is not None:
@@ -50,7 +51,7 @@ def _ref(q, k, v, do, scale, mask=None, dlse=None):
     A, C = do.abs() @ v.abs().transpose(2, 3), (do.abs() * out.abs()).sum(-1, keepdim=True)
     if dlse is not None:
         C = C + dlse.double().abs()[..., None]
-    err = (u + 2.0 ** -14 + 2.0 ** -17) * ds.abs() + p * (u * C + 2.0 ** -17 * (A + C))
+    err = (u + 2.0 ** -14 + 2.0 ** -17) * ds.abs() + p * (u_out * C + 2.0 ** -17 * (A + C))
     tol = (scale * err @ k.abs(), scale * err.transpose(2, 3) @ q.abs(),
            (u + 2.0 ** -14 + 2.0 ** -17) * p.transpose(2, 3) @ do.abs())
     return out, lse, grads, tol
@@ -203,6 +204,36 @@ def test_flat_and_peaked_scores(qscale, dtype):
     """Equal scores, and scores of a deviation of 8 (fp32 rounds those to 2^-18: the 2^-14 of the
     tolerance holds up to 2^4 units times 16 terms' worth of rounding)."""
     _run(*_tensors(1, 2, 150, 300, 64, dtype, False, qscale=qscale))
+
+
+@pytest.mark.parametrize("Skv", [2, 3, 17, 63, 64])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("with_dlse", [False, True])
+def test_few_keys_do_not_see_the_rounding_of_out(Skv, D, with_dlse):
+    """bf16 with up to 64 keys: delta is formed from P and dP, so that its error is that of fp32 sums
+    (2^-14 P as in P itself), not that of out's rounding."""
+    q, k, v, do = _tensors(1, 3, 200, Skv, D, BF, True, qscale=2.0)
+    scale = D ** -0.5
+    dlse = torch.randn((1, 3, 200), generator=torch.Generator().manual_seed(1)).cuda() if with_dlse else None
+    out, lse, grads, tol = _ref(q, k, v, do, scale, None, dlse, u_out=2.0 ** -14)
+    got = ops.flash_bwd(q, k, v, out.to(BF), lse.float(), do, scale, dlse)
+    _check(got, grads, tol, BF)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("sparse", [False, True])
+def test_one_key(dtype, sparse):
+    """The softmax of one key does not depend on q and k: their gradients are exactly zero, and with a
+    gradient of the LSE its own."""
+    q, k, v, do = _tensors(2, 2, 150, 1, 128, dtype, False)
+    tiles = None
+    if sparse:
+        m = torch.ones((2, 3, 1), dtype=torch.bool, device="cuda")
+        tiles = ops.mask_to_tiles(m, 64, union_rows=False)
+    got = _run(q, k, v, do, tiles=tiles)
+    assert (got[0] == 0).all() and (got[1] == 0).all()
+    dlse = torch.randn((2, 2, 150), generator=torch.Generator().manual_seed(1)).cuda()
+    _run(q, k, v, do, tiles=tiles, dlse=dlse)
 
 
 def test_non_finite_values_stay_where_no_pair_reaches():

@@ -6,6 +6,7 @@ Nothing in this module computes on the host, and nothing falls back to torch mat
 """
 from __future__ import annotations
 
+import contextlib
 import functools
 import math
 import warnings
@@ -35,7 +36,8 @@ def _require_gpu(*tensors: torch.Tensor, what: str) -> None:
 
 def _kernel_strides(t: torch.Tensor) -> bool:
     """Whether the kernels can address (B,H,S,D) t: unit dim stride, 16-byte aligned rows."""
-    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in t.stride()[:3])
+    sb, sh, ss, sd = t.stride()
+    return sd == 1 and not (sb | sh | ss) % 8 and t.data_ptr() % 16 == 0
 
 
 def _attn_view(t: torch.Tensor) -> torch.Tensor:
@@ -237,7 +239,7 @@ def transpose_tiles(tiles: TileList, kv_len: int) -> KeyTileList:
     nk = (int(kv_len) - tiles.origin + 127) // 128
     out = KeyTileList(torch.empty((H, nk), device=device, dtype=torch.int32),
                       torch.empty((H, nk, 2 * nq), device=device, dtype=torch.int32), int(tiles.origin))
-    with torch.cuda.device(device):
+    with _on(device):
         check(_lib.load().moddit_transpose_tiles(
             tiles.counts.data_ptr(), tiles.entries.data_ptr(), H, nq, tiles.cap, out.counts.data_ptr(),
             out.entries.data_ptr(), nk, out.cap, _stream(tiles.counts)), "moddit_transpose_tiles")
@@ -263,7 +265,7 @@ def _attention_bwd(what, q, k, v, out, lse, grad_out, scale, grad_lse, tiles, ke
     if out.shape != q.shape or grad_out.shape != q.shape:
         raise ValueError(f"{what}: out and grad_out must have query's shape {tuple(q.shape)}, got "
                          f"{tuple(out.shape)} and {tuple(grad_out.shape)}")
-    if any(t.dtype != q.dtype for t in (k, v, out, grad_out)):
+    if not (q.dtype == k.dtype == v.dtype == out.dtype == grad_out.dtype):
         raise ValueError(f"{what}: query, key, value, out and grad_out must have the same dtype")
     dt = _attn_dtype(q)
     B, H, Sq, D = q.shape
@@ -288,9 +290,9 @@ def _attention_bwd(what, q, k, v, out, lse, grad_out, scale, grad_lse, tiles, ke
         if key_tiles.counts.shape[0] != H or key_tiles.origin != origin or key_tiles.cap != 2 * tiles.n_qtiles:
             raise ValueError(f"{what}: key_tiles are not the transposed lists of tiles")
     # rows of one token expanded along the sequence are stored out: the kernels tell rows by address
-    q, k, v, out, grad_out = (_attn_view(t if t.shape[2] < 2 or t.stride(2) >= D else t.contiguous())
-                              for t in (q, k, v, out, grad_out))
-    lse, grad_lse = (None if t is None else t.contiguous() for t in (lse, grad_lse))
+    q, k, v, out, grad_out = [_attn_view(t if t.shape[2] < 2 or t.stride(2) >= D else t.contiguous())
+                              for t in (q, k, v, out, grad_out)]
+    lse, grad_lse = [None if t is None else t.contiguous() for t in (lse, grad_lse)]
     dq, dk, dv = _empty_as(q), _empty_as(k), _empty_as(v)
     lib = _lib.load()
     nbytes = _split_bytes("moddit_attention_bwd_workspace_bytes", B, H, Sq, Skv, D, dt, origin,
@@ -298,9 +300,9 @@ def _attention_bwd(what, q, k, v, out, lse, grad_out, scale, grad_lse, tiles, ke
     ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
     args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), grad_out.data_ptr(),
             _ptr(grad_lse), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, H, Sq, Skv, D,
-            *(strides3(*t.stride()[:3]) for t in (q, k, v, out, grad_out, dq, dk, dv)),
+            *[strides3(*t.stride()[:3]) for t in (q, k, v, out, grad_out, dq, dk, dv)],
             float(D ** -0.5 if scale is None else scale), dt)
-    with torch.cuda.device(device):
+    with _on(device):
         if tiles is None:
             check(lib.moddit_flash_bwd(*args, ws.data_ptr(), nbytes, _stream(q)), "moddit_flash_bwd")
         else:
@@ -333,13 +335,23 @@ _WEIGHT_DTYPES = {**_DTYPES, torch.float32: _lib.FP32}
 _MAX_NORM_ROW = 8192
 
 
-def _same_device(what, *tensors):
+def _same_device(what, first, *others):
     """All tensors (None aside) on the first one's GPU, which is returned."""
-    got = [t for t in tensors if t is not None]
-    _require_gpu(*got, what=what)
-    if any(t.device != got[0].device for t in got):
-        raise ValueError(f"{what}: tensors must live on the same GPU")
-    return got[0].device
+    device = first.device
+    for t in (first, *others):
+        if t is not None:
+            if not t.is_cuda:
+                raise ValueError(f"{what}: tensors must live on a GPU (got {t.device})")
+            if t.device != device:
+                raise ValueError(f"{what}: tensors must live on the same GPU")
+    return device
+
+
+def _on(device):
+    """A context with `device` current: launches go to its streams."""
+    if torch.cuda.current_device() == device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def _qk_norm_args(what, q, k, norm, across_heads, eps, weights, biases, cos, sin, rope_offset):
@@ -420,10 +432,10 @@ def qk_norm_rope(q, k, *, norm="rms", across_heads=False, eps=1e-6, q_weight=Non
                 raise ValueError(f"{what}: out needs a unit dim stride, 16-byte alignment and strides of "
                                  "multiples of 8 elements")
     q, k = _attn_view(q), _attn_view(k)
-    with torch.cuda.device(device):
+    with _on(device):
         check(_lib.load().moddit_qk_norm_rope(
             q.data_ptr(), k.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), *sizes,
-            *(strides3(*t.stride()[:3]) for t in (q, k, *out)), _attn_dtype(q), *head,
+            *[strides3(*t.stride()[:3]) for t in (q, k, *out)], _attn_dtype(q), *head,
             _ptr(w[0]), _ptr(w[1]), _ptr(b[0]), _ptr(b[1]), w_dt, *tables, int(bool(interleaved)),
             _stream(q)), "moddit_qk_norm_rope")
     return out
@@ -453,11 +465,11 @@ def qk_norm_rope_bwd(q, k, grad_q, grad_k, *, norm="rms", across_heads=False, ep
     if any(t is not None for t in sums) and not empty:
         floats = lib.moddit_qk_norm_rope_bwd_workspace_floats(*sizes, head[1])
         ws = torch.empty(floats, device=device, dtype=torch.float32)
-    with torch.cuda.device(device):
+    with _on(device):
         check(lib.moddit_qk_norm_rope_bwd(
             q.data_ptr(), k.data_ptr(), grad_q.data_ptr(), grad_k.data_ptr(), dq.data_ptr(), dk.data_ptr(),
             *(_ptr(t) for t in sums), *sizes,
-            *(strides3(*t.stride()[:3]) for t in (q, k, grad_q, grad_k, dq, dk)), _attn_dtype(q), *head,
+            *[strides3(*t.stride()[:3]) for t in (q, k, grad_q, grad_k, dq, dk)], _attn_dtype(q), *head,
             _ptr(w[0]), _ptr(w[1]), w_dt, *tables, int(bool(interleaved)), _ptr(ws), floats, _stream(q)),
             "moddit_qk_norm_rope_bwd")
     return (dq, dk, *sums)

@@ -97,6 +97,10 @@ __device__ __forceinline__ void store_row(uint16_t* row, int l, int dim, u32x4 v
   }
 }
 
+// x, unpacked again from here on: else the compiler keeps the fp32 values of one pass over a row for
+// the next, twice the registers of the row itself.
+__device__ __forceinline__ void repack(u32x4& x) { asm volatile("" : "+v"(x)); }
+
 template <typename E>
 __device__ __forceinline__ void unpack(u32x4 v, float (&f)[8]) {
 #pragma unroll
@@ -105,10 +109,10 @@ __device__ __forceinline__ void unpack(u32x4 v, float (&f)[8]) {
 
 template <typename E>
 __device__ __forceinline__ u32x4 pack(const float (&f)[8]) {
-  u32x4 v;
+  typename E::vec8 v;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = pack2(E::from_float(f[2 * i]), E::from_float(f[2 * i + 1]));
-  return v;
+  for (int i = 0; i < 8; ++i) v[i] = static_cast<typename E::elem>(f[i]);  // to nearest even
+  return __builtin_bit_cast(u32x4, v);
 }
 
 __device__ __forceinline__ float affine_at(const void* w, int type, int64_t i, float none) {
@@ -351,6 +355,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_wave_kernel(RopeParams p) 
     }
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
+      if (kNorm == kLayer) repack(raw[j]);
       float x[8], part = 0.f;
       unpack<E>(raw[j], x);
 #pragma unroll
@@ -362,6 +367,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_wave_kernel(RopeParams p) 
     for (int j = 0; j < kChunks; ++j) {
       const int ch = lane + 64 * j;
       if (ch >= n_chunks) break;
+      repack(raw[j]);
       float y[8];
       unpack<E>(raw[j], y);
       const f32x4 w[2] = {*reinterpret_cast<const f32x4*>(affine + 4 * ch),

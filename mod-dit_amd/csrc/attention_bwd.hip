@@ -51,6 +51,9 @@ __device__ __forceinline__ u32x4 lds_read16(uint32_t a) {
   return *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(a);
 }
 
+// Entries of a block-sparse list that are arranged in LDS at a time (two per thread).
+constexpr int kListChunk = 2 * kThreads;
+
 // At D = 128 the dK/dV pass has no registers for V beside its sums (128) and K (32): V stays in
 // LDS, and stages are half a tile so that two workgroups fit a CU.
 template <int D, bool kKeys>
@@ -64,7 +67,8 @@ struct BwdLds {
   static constexpr int kWinPerWave = kTileBytes / 1024 / 4;
   static constexpr int kStage = 2 * kTileBytes + (kKeys ? kStatsBytes : 0);
   static constexpr int kOwn2Bytes = kOwn2InLds ? kBM * kRowBytes : 0;
-  static constexpr int kTotal = 2 * kStage + kOwn2Bytes;
+  static constexpr int kSteps0 = 2 * kStage + kOwn2Bytes;  // where a block-sparse list's steps lie
+  static constexpr int kTotal = kSteps0 + (kSteps == 1 ? kListChunk * 8 : 0);
 };
 
 // XOR on the 16-byte chunks of LDS row r. Both reads of a tile are free of bank conflicts: the
@@ -324,6 +328,16 @@ __device__ __forceinline__ int ds_exponent(const float* maxima, int n, float (*r
   return e < -100 ? -100 : (e > 100 ? 100 : e);
 }
 
+// What a stage holds and who computes on it. With kSteps == 1 a stage has two slots of 32 rows: the
+// halves of tile a, for the halves of the owned rows whose bits are set in `halves`; or, with none
+// set, half `part` of tile a for the first half of the owned rows and of tile b for the second: list
+// entries that one half uses go in pairs, and neither half waits while the other works (a third of a
+// random mask's work: dQ of 28,800 tokens x 12 heads, 19 % kept at random, D = 128: see PAIRED).
+// With kSteps == 2 a stage is half `part` of tile a.
+struct Step {
+  int a, b, part, halves;
+};
+
 // Workgroup `wg` of one pass.
 template <int D, typename E, bool kKeys, bool kSparse>
 __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) {
@@ -332,6 +346,7 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
   constexpr int kKC = D / 32;  // MFMA k-steps over d
   constexpr int kDB = D / 16;  // 16-row blocks of the transposed sums
   constexpr bool kHalf = std::is_same<E, Fp16>::value;
+  constexpr bool kPaired = kSparse && L::kSteps == 1;
 
   extern __shared__ __align__(16) unsigned char smem[];
   const int tid = threadIdx.x;
@@ -366,8 +381,9 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
     else
       it0 = first;
   }
+  const int slot = __builtin_amdgcn_readfirstlane(wave) >> 1;  // the half of the owned rows this wave lies in
   const int first_row = p.origin + ot * kBM + __builtin_amdgcn_readfirstlane(wave) * 32;
-  const int wbit = first_row < p.own_len && first_row + 31 >= 0 ? 1 << (wave >> 1) : 0;
+  const int wbit = first_row < p.own_len && first_row + 31 >= 0 ? 1 << slot : 0;
 
   const float* stats = p.stats + static_cast<int64_t>(bh) * p.stat_blocks * 128;
   // ---- staging, as in the forward: window w of a tile holds LDS bytes [1024 w, +1024) ----
@@ -385,18 +401,25 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
     src1[i] = static_cast<uint32_t>(((p.origin + r) * static_cast<int>(p.str1.ss) + ch * 8) * 2);
     src2[i] = static_cast<uint32_t>(((p.origin + r) * static_cast<int>(p.str2.ss) + ch * 8) * 2);
   }
-  const uint32_t step1 = static_cast<uint32_t>(L::kRows * p.str1.ss * 2);
-  const uint32_t step2 = static_cast<uint32_t>(L::kRows * p.str2.ss * 2);
-  auto dma = [&](int st, int part, int stage) {
+  const uint32_t row1 = static_cast<uint32_t>(p.str1.ss * 2), row2 = static_cast<uint32_t>(p.str2.ss * 2);
+  auto dma = [&](const Step& x, int stage) {
     const uint32_t dst = lds0 + stage * L::kStage;
-    const uint32_t at = st * L::kSteps + part;
+    uint32_t row = x.a * kBN + (L::kSteps == 1 ? 0 : x.part * 32);
+    if (kPaired && x.halves == 0)  // waves 0 and 1 fill slot 0, the others slot 1
+      row = slot == 0 ? x.a * kBN + x.part * 32 : x.b * kBN + x.part * 32 - 32;
 #pragma unroll
     for (int i = 0; i < L::kWinPerWave; ++i)
-      lds_dma16(rsrc1, dst + (wave * L::kWinPerWave + i) * 1024, src1[i] + at * step1, 0);
+      lds_dma16(rsrc1, dst + (wave * L::kWinPerWave + i) * 1024, src1[i] + row * row1, 0);
 #pragma unroll
     for (int i = 0; i < L::kWinPerWave; ++i)
-      lds_dma16(rsrc2, dst + L::kTileBytes + (wave * L::kWinPerWave + i) * 1024, src2[i] + at * step2, 0);
-    if (kKeys && wave == 0) lds_dma16(rsrc_st, dst + 2 * L::kTileBytes, lane * 16 + st * 512, 0);
+      lds_dma16(rsrc2, dst + L::kTileBytes + (wave * L::kWinPerWave + i) * 1024, src2[i] + row * row2, 0);
+    if (kKeys && wave == 0) {
+      // 16 lanes of -LSE, 16 of -delta, 8 of each per slot; the others load what nobody reads
+      uint32_t off = lane * 16 + x.a * 512;
+      if (kPaired && x.halves == 0)
+        off = ((lane & 8) ? x.b : x.a) * 512 + ((lane & 16) ? 256 : 0) + x.part * 128 + (lane & 7) * 16;
+      lds_dma16(rsrc_st, dst + 2 * L::kTileBytes, off, 0);
+    }
   };
   if constexpr (L::kOwn2InLds) {
     const int64_t span = (static_cast<int64_t>(p.own_len) - 1) * p.own2.ss * 2 + L::kRowBytes;
@@ -411,18 +434,75 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
     }
   }
 
-  auto decode = [&](int e_raw, int& st, int& flags) {
-    const int e = __builtin_amdgcn_readfirstlane(e_raw);
-    st = e >> 2;
-    flags = (st >= 0 && st < p.n_str_tiles) ? (e & 3) : 0;  // as in the forward
-    st = st < 0 ? 0 : (st < p.n_str_tiles ? st : p.n_str_tiles - 1);
+  // An entry outside the grid's streamed tiles is executed by no wave, as in the forward.
+  auto rows_bits = [&](int e) { return (e >> 2) >= 0 && (e >> 2) < p.n_str_tiles ? e & 3 : 0; };
+  auto arrange = [&](int first) -> int {
+    if constexpr (!kPaired) return n_iter * L::kSteps;
+    __shared__ int count[kThreads / 64][4];
+    u32x2* const steps = reinterpret_cast<u32x2*>(smem + L::kSteps0);
+    int e[2], f[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i = first + 2 * tid + u;
+      e[u] = i < n_iter ? list[i] : 0;
+      f[u] = i < n_iter ? rows_bits(e[u]) : 0;
+    }
+    const uint64_t below = (1ull << lane) - 1;
+    int rank[2] = {0, 0};
+#pragma unroll
+    for (int k = 1; k < 4; ++k) {
+      const uint64_t m0 = __ballot(f[0] == k), m1 = __ballot(f[1] == k);
+      const int before = __builtin_popcountll(m0 & below) + __builtin_popcountll(m1 & below);
+      if (f[0] == k) rank[0] = before;
+      if (f[1] == k) rank[1] = before + (f[0] == k);
+      if (lane == 0) count[wave][k] = __builtin_popcountll(m0) + __builtin_popcountll(m1);
+    }
+    __syncthreads();
+    int total[4] = {0, 0, 0, 0}, mine[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w)
+#pragma unroll
+      for (int k = 1; k < 4; ++k) {
+        if (w < wave) mine[k] += count[w][k];
+        total[k] += count[w][k];
+      }
+    const int pairs = total[1] < total[2] ? total[1] : total[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint32_t t = static_cast<uint32_t>(e[u] >> 2);
+      const int r = rank[u] + (f[u] == 1 ? mine[1] : f[u] == 2 ? mine[2] : mine[3]);
+      if (f[u] == 3) {
+        steps[r] = u32x2{t | (3u << 30), t};
+      } else if (f[u] != 0 && r >= pairs) {
+        steps[total[3] + pairs + r] = u32x2{t | (static_cast<uint32_t>(f[u]) << 30), t};
+      } else if (f[u] == 1) {
+        steps[total[3] + 2 * r].x = steps[total[3] + 2 * r + 1].x = t;
+      } else if (f[u] == 2) {
+        steps[total[3] + 2 * r].y = t;
+        steps[total[3] + 2 * r + 1].y = t | (1u << 31);
+      }
+    }
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(total[3] + total[1] + total[2]);
   };
-  auto entry = [&](int i) -> int { return kSparse ? list[i] : (((it0 + i) << 2) | 3); };
+  auto step_at = [&](int j) -> Step {
+    if constexpr (kPaired) {
+      const u32x2 x = reinterpret_cast<const u32x2*>(smem + L::kSteps0)[j];
+      const uint32_t a = __builtin_amdgcn_readfirstlane(x.x), b = __builtin_amdgcn_readfirstlane(x.y);
+      return Step{static_cast<int>(a & 0x3fffffffu), static_cast<int>(b & 0x7fffffffu), static_cast<int>(b >> 31), static_cast<int>(a >> 30)};
+    } else {
+      const int i = j / L::kSteps;
+      const int e = kSparse ? __builtin_amdgcn_readfirstlane(list[i]) : (((it0 + i) << 2) | 3);
+      const int t = e >> 2 < 0 ? 0 : (e >> 2 < p.n_str_tiles ? e >> 2 : p.n_str_tiles - 1);
+      return Step{t, t, j % L::kSteps, rows_bits(e)};
+    }
+  };
   // the first stage is on its way while the owned rows are read
-  int st = 0, flags = 0;
-  if (n_iter > 0) {
-    decode(entry(0), st, flags);
-    dma(st, 0, 0);
+  int n_steps = arrange(0);
+  Step now{0, 0, 0, 0};
+  if (n_steps > 0) {
+    now = step_at(0);
+    dma(now, 0);
   }
 
   float ds_scale = 1.f;  // fp16: from P (dQ pass) or 2^15 P to 2^e dS
@@ -640,34 +720,42 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
     }
   __builtin_amdgcn_s_waitcnt(0);  // V's DMA too, which must not outlive the workgroup
   __syncthreads();
-  const int n_steps = n_iter * L::kSteps;
   // A step whose stage is known to the compiler: operand addresses are immediates of its reads.
-  auto step = [&](int j, auto stage_of_j) {
+  auto run = [&](int j, auto stage_of_j) {
     constexpr int kStageOff = decltype(stage_of_j)::value * L::kStage;
-    const int part = j % L::kSteps;
-    int st1 = st, flags1 = flags;
+    Step next = now;
     if (j + 1 < n_steps) {
-      if (part == L::kSteps - 1) decode(entry((j + 1) / L::kSteps), st1, flags1);
-      dma(st1, (j + 1) % L::kSteps, 1 - decltype(stage_of_j)::value);
+      next = step_at(j + 1);
+      dma(next, 1 - decltype(stage_of_j)::value);
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (flags & wbit) {
-      if constexpr (L::kSteps == 1) {
-        half_tile(kStageOff, kStageOff);
-        __builtin_amdgcn_sched_barrier(0);
-        half_tile(kStageOff + 32 * L::kRowBytes, kStageOff + 128);
-      } else {
-        half_tile(kStageOff, kStageOff + 128 * part);
-      }
+    const bool both = (now.halves & wbit) != 0, paired = kPaired && now.halves == 0 && wbit != 0;
+    if constexpr (L::kSteps == 1) {
+      if (both || (paired && slot == 0)) half_tile(kStageOff, kStageOff);
+      __builtin_amdgcn_sched_barrier(0);
+      if (both || (paired && slot == 1)) half_tile(kStageOff + 32 * L::kRowBytes, kStageOff + 128);
+    } else {
+      if (both) half_tile(kStageOff, kStageOff + 128 * now.part);
     }
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    st = st1;
-    flags = flags1;
+    now = next;
   };
-  for (int j = 0; j < n_steps; j += 2) {
-    step(j, std::integral_constant<int, 0>{});
-    if (j + 1 < n_steps) step(j + 1, std::integral_constant<int, 1>{});
+  for (int first = 0;;) {
+    for (int j = 0; j < n_steps; j += 2) {
+      run(j, std::integral_constant<int, 0>{});
+      if (j + 1 < n_steps) run(j + 1, std::integral_constant<int, 1>{});
+    }
+    if constexpr (!kPaired) break;
+    first += kListChunk;
+    if (first >= n_iter) break;
+    n_steps = arrange(first);
+    if (n_steps > 0) {
+      now = step_at(0);
+      dma(now, 0);
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
   }
 
   if (split) {

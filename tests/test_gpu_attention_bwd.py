@@ -154,6 +154,18 @@ def test_sparse_with_more_queries_than_keys_and_batch():
     _run(q, k, v, do, mask=mask, tiles=tiles)
 
 
+@pytest.mark.parametrize("D,dtype", [(64, FP), (128, BF)])
+@pytest.mark.parametrize("rows,keys", [(190, 70 * 640), (70 * 640, 150)])
+def test_lists_of_many_entries(D, dtype, rows, keys):
+    """Lists longer than a workgroup arranges at a time, most of their entries for one half alone."""
+    g = torch.Generator().manual_seed(6)
+    m = (torch.rand((1, -(-rows // 64), -(-keys // 64)), generator=g) < 0.6).cuda()
+    tiles = ops.mask_to_tiles(m, 64, union_rows=False)
+    q, k, v, do = _tensors(1, 1, rows, keys, D, dtype, False)
+    mask = m.repeat_interleave(64, 1).repeat_interleave(64, 2)[None, :, :rows, :keys]
+    _run(q, k, v, do, mask=mask, tiles=tiles)
+
+
 @pytest.mark.parametrize("H,nq,nk,p", [(1, 1, 1, 1.0), (2, 5, 3, 0.5), (3, 40, 70, 0.1), (1, 7, 33, 0.0), (2, 130, 64, 0.9)])
 def test_transpose_tiles(H, nq, nk, p):
     """Every (query block, key tile) pair of the lists, and no other, in ascending order."""

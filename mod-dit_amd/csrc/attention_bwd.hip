@@ -71,12 +71,15 @@ struct BwdLds {
   static constexpr int kTotal = kSteps0 + (kSteps == 1 ? kListChunk * 8 : 0);
 };
 
-// XOR on the 16-byte chunks of LDS row r. Both reads of a tile are free of bank conflicts: the
-// 16 rows of a row read lie in 16 different chunks of 256 bytes, and so do the 8 rows x 2 chunks
-// of a half wave's transposed read.
+// XOR on the 16-byte chunks of LDS row r that keeps both reads of a tile free of bank conflicts (64
+// banks). A transposed read's half wave takes two neighbouring chunks of 8 rows: they lie in 16
+// different chunks of 256 bytes. A row read's 16 lanes of a cycle are rows 0-3 and 12-15 of one chunk
+// and rows 4-11 of its neighbour (or the others): these are 16 different ones too, as long as the XOR is
+// even. With one that differs in its last bit between rows 0-7 and 8-15 37 % of the LDS cycles were
+// conflicts.
 template <int D>
 __device__ __forceinline__ int swz(int r) {
-  return D == 128 ? 2 * (r & 7) + ((r >> 3) & 1) : 2 * ((r >> 1) & 3) + ((r >> 3) & 1);
+  return 2 * ((r / (128 / D)) % (D / 16));
 }
 
 // x, in registers from here on.

@@ -387,7 +387,7 @@ int moddit_flash_bwd(const void* q, const void* k, const void* v, const void* o,
  * (key_counts, key_entries) the same pairs by key tile, from moddit_transpose_tiles: for head h and
  * the 128 grid keys of tile t < n_ktiles = ceil((kv_len - grid_origin) / 128) the query blocks of 64
  * rows that attend to it, ascending, each as (query block << 2) | keys, bit 0 for keys 0..63 of the
- * tile and bit 1 for keys 64..127.
+ * tile and bit 1 for keys 64..127. Without queries or without keys the lists are not read.
  */
 int moddit_block_sparse_bwd(const void* q, const void* k, const void* v, const void* o,
                             const float* lse, const void* grad_o, const float* grad_lse, void* dq,

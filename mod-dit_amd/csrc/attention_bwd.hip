@@ -334,9 +334,10 @@ __device__ __forceinline__ int ds_exponent(const float* maxima, int n, float (*r
 // What a stage holds and who computes on it. With kSteps == 1 a stage has two slots of 32 rows: the
 // halves of tile a, for the halves of the owned rows whose bits are set in `halves`; or, with none
 // set, half `part` of tile a for the first half of the owned rows and of tile b for the second: list
-// entries that one half uses go in pairs, and neither half waits while the other works (a third of a
-// random mask's work: dQ of 28,800 tokens x 12 heads, 19 % kept at random, D = 128: see PAIRED).
-// With kSteps == 2 a stage is half `part` of tile a.
+// entries that one half uses go in pairs, and neither half waits while the other works (random masks:
+// 17,776 tokens x 16 heads, D = 64 1.84 -> 1.76 ms; 7,680 x 12, D = 128, where only the dQ pass has them,
+// 521 -> 493 us). With kSteps == 2 a stage is half `part` of tile a: two slots of 32 rows would not fit
+// beside V with two workgroups to a CU.
 struct Step {
   int a, b, part, halves;
 };
@@ -1069,6 +1070,7 @@ struct BwdArgs {
   const int64_t *qs, *ks, *vs, *os, *ds, *dqs, *dks, *dvs;
   float scale;
   int dtype;
+  bool sparse;
   const int32_t *counts, *entries;
   int n_qtiles, cap;
   const int32_t *key_counts, *key_entries;
@@ -1102,10 +1104,12 @@ int bwd_entry(const BwdArgs& a, moddit_stream_t stream) {
     return MODDIT_EUNSUPPORTED;
   }
   MODDIT_CHECK_ARG(a.origin > -kBN && a.origin <= 0, "attention_bwd: grid_origin must be in (-64, 0], got %d", a.origin);
-  const bool sparse = a.counts != nullptr;
+  // the lists of an empty side name no row, and are not looked at
+  const bool lists = a.sparse && a.q_len > 0 && a.kv_len > 0;
   const int64_t nq = (static_cast<int64_t>(a.q_len) - a.origin + kBM - 1) / kBM;
   const int64_t nk = (static_cast<int64_t>(a.kv_len) - a.origin + kBM - 1) / kBM;
-  if (sparse) {
+  if (lists) {
+    MODDIT_CHECK_ARG(a.counts, "attention_bwd: counts must not be NULL");
     MODDIT_CHECK_ARG(a.entries && a.key_counts && a.key_entries, "attention_bwd: tile lists missing");
     MODDIT_CHECK_ARG(a.n_qtiles == nq, "attention_bwd: n_qtiles=%d but q_len=%d (grid origin %d) needs %lld", a.n_qtiles,
                      a.q_len, a.origin, static_cast<long long>(nq));
@@ -1119,7 +1123,6 @@ int bwd_entry(const BwdArgs& a, moddit_stream_t stream) {
                    "attention_bwd: null tensor pointer");
   const void* all[8] = {a.q, a.k, a.v, a.o, a.d, a.dq, a.dk, a.dv};
   for (const void* t : all) MODDIT_CHECK_ARG(aligned16(t), "attention_bwd: tensors must be 16-byte aligned");
-  const bool lists = sparse && a.q_len > 0 && a.kv_len > 0;  // an empty side's lists name no row
   const BwdPlan plan = plan_bwd(a.batch, a.heads, a.q_len, a.kv_len, a.head_dim, a.dtype, a.origin, lists ? a.cap : 0,
                                 lists ? a.key_cap : 0);
   const int64_t need = plan.total * 4;
@@ -1307,7 +1310,7 @@ extern "C" int moddit_flash_bwd(const void* q, const void* k, const void* v, con
                                 int64_t workspace_bytes, moddit_stream_t stream) {
   const moddit::BwdArgs a{q, k, v, o, grad_o, lse, grad_lse, dq, dk, dv, batch, heads, q_len, kv_len, head_dim,
                           q_strides, k_strides, v_strides, o_strides, go_strides, dq_strides, dk_strides, dv_strides,
-                          softmax_scale, dtype, nullptr, nullptr, 0, 0, nullptr, nullptr, 0, 0, 0, workspace,
+                          softmax_scale, dtype, false, nullptr, nullptr, 0, 0, nullptr, nullptr, 0, 0, 0, workspace,
                           workspace_bytes};
   return moddit::bwd_entry(a, stream);
 }
@@ -1323,14 +1326,10 @@ extern "C" int moddit_block_sparse_bwd(const void* q, const void* k, const void*
                                        const int32_t* key_counts, const int32_t* key_entries, int n_ktiles,
                                        int key_cap, int grid_origin, void* workspace, int64_t workspace_bytes,
                                        moddit_stream_t stream) {
-  if (counts == nullptr) {
-    moddit::set_error("block_sparse_bwd: counts must not be NULL");
-    return MODDIT_EINVAL;
-  }
   const moddit::BwdArgs a{q, k, v, o, grad_o, lse, grad_lse, dq, dk, dv, batch, heads, q_len, kv_len, head_dim,
                           q_strides, k_strides, v_strides, o_strides, go_strides, dq_strides, dk_strides, dv_strides,
-                          softmax_scale, dtype, counts, entries, n_qtiles, cap, key_counts, key_entries, n_ktiles,
-                          key_cap, grid_origin, workspace, workspace_bytes};
+                          softmax_scale, dtype, true, counts, entries, n_qtiles, cap, key_counts, key_entries,
+                          n_ktiles, key_cap, grid_origin, workspace, workspace_bytes};
   return moddit::bwd_entry(a, stream);
 }
 

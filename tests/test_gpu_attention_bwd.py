@@ -304,6 +304,11 @@ def test_empty_sides(Sq, Skv, dtype):
     lse = torch.full((1, 2, Sq), float("-inf"), device="cuda")
     for t in ops.flash_bwd(q, k, v, do, lse, do):
         assert (t == 0).all()
+    nq, cap = (Sq + 127) // 128, (Skv + 63) // 64
+    tiles = ops.TileList(torch.zeros((2, nq), dtype=torch.int32, device="cuda"),
+                         torch.zeros((2, nq, cap), dtype=torch.int32, device="cuda"), 64, False)
+    for t, x in zip(ops.block_sparse_bwd(q, k, v, do, lse, do, tiles), (q, k, v)):
+        assert t.shape == x.shape and (t == 0).all()
 
 
 def test_gradients_against_differences():

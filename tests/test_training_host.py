@@ -108,6 +108,7 @@ def test_attention_bwd_refuses(kw, rc, word):
 def test_attention_bwd_of_nothing_is_done_without_a_launch():
     assert _bwd(q=None, sizes=(1, 0, 64, 64, 64)) == _lib.MODDIT_OK
     assert _bwd(q=None, sizes=(1, 2, 0, 0, 64), ws=None) == _lib.MODDIT_OK
+    assert _bwd(sparse=True, q=None, sizes=(1, 2, 0, 0, 64), lists=(None, None, 0, 0) * 2, ws=None) == _lib.MODDIT_OK
 
 
 def test_transpose_tiles_refuses():

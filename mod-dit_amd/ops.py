@@ -431,6 +431,13 @@ def qk_norm_rope(q, k, *, norm="rms", across_heads=False, eps=1e-6, q_weight=Non
             if not _kernel_strides(t):
                 raise ValueError(f"{what}: out needs a unit dim stride, 16-byte alignment and strides of "
                                  "multiples of 8 elements")
+        for t, x, others in ((q_out, q, (k, k_out)), (k_out, k, (q, q_out))):
+            long = [i for i in range(3) if t.shape[i] > 1]
+            if t.numel() and (any(t.stride(i) == 0 for i in long) or
+                              any(t.data_ptr() == y.data_ptr() for y in others) or
+                              t.data_ptr() == x.data_ptr() and any(t.stride(i) != x.stride(i) for i in long)):
+                raise ValueError(f"{what}: the tensors of out must lie apart from each other and, unless they "
+                                 "are q and k themselves, from both")
     q, k = _attn_view(q), _attn_view(k)
     with _on(device):
         check(_lib.load().moddit_qk_norm_rope(

@@ -323,6 +323,11 @@ def test_refusals():
         (ValueError, "exceed", dict(rope_offset=-1)),
         (ValueError, "GPU", dict(q_weight=kw["q_weight"].cpu())),
         (ValueError, "out must be", dict(out=(q, k[:, :1]))),
+        (ValueError, "apart", dict(out=(k, q))),
+        (ValueError, "apart", dict(out=(q, q))),
+        (ValueError, "apart", dict(out=(q, torch.empty_like(k[:, :1]).expand(-1, 2, -1, -1)))),
+        (ValueError, "apart", dict(k=q, out=(q, k.clone()))),
+        (ValueError, "apart", dict(out=(q.view(1, 16, 2, 64).transpose(1, 2), k))),
         (ValueError, "unit dim stride", dict(out=(q.transpose(2, 3).contiguous().transpose(2, 3), k.clone()))),
     ]
     for error, word, change in cases:

@@ -54,21 +54,31 @@ __device__ __forceinline__ u32x4 lds_read16(uint32_t a) {
 // Entries of a block-sparse list that are arranged in LDS at a time (two per thread).
 constexpr int kListChunk = 2 * kThreads;
 
-// At D = 128 the dK/dV pass has no registers for V beside its sums (128) and K (32): V stays in
-// LDS, and stages are half a tile so that two workgroups fit a CU.
-template <int D, bool kKeys>
+// At D = 128 the dK/dV pass has no registers for V beside its sums (128) and K (32): V stays in LDS,
+// as MFMA operands of 1 KB, and stages are half a tile so that two workgroups fit a CU.
+//
+// Its block-sparse form owns one 64-key tile (kOneTile): an entry of a list by 128 keys names both
+// halves of the keys less than half the time (random masks), and waves of the other half would wait.
+// Two waves take the first 32 rows of each streamed tile and two the others, with sums that are added
+// at the end. One operand of V a wave is held in registers so that this fits 80 KB.
+template <int D, bool kKeys, bool kSparse>
 struct BwdLds {
   static constexpr bool kOwn2InLds = kKeys && D == 128;
-  static constexpr int kRows = kOwn2InLds ? 32 : kBN;  // streamed rows of a stage
+  static constexpr bool kOneTile = kOwn2InLds && kSparse;
+  static constexpr int kOwn = kOneTile ? 64 : kBM;     // owned rows
+  static constexpr int kRows = kOwn2InLds && !kOneTile ? 32 : kBN;  // streamed rows of a stage
   static constexpr int kSteps = kBN / kRows;           // stages of a tile
+  static constexpr bool kPaired = kSparse && kSteps == 1 && !kOneTile;  // see Step
   static constexpr int kRowBytes = D * 2;
   static constexpr int kTileBytes = kRows * kRowBytes;  // one tensor's part of a stage
   static constexpr int kRowsPerWindow = 1024 / kRowBytes;
   static constexpr int kWinPerWave = kTileBytes / 1024 / 4;
-  static constexpr int kStage = 2 * kTileBytes + (kKeys ? kStatsBytes : 0);
-  static constexpr int kOwn2Bytes = kOwn2InLds ? kBM * kRowBytes : 0;
+  static constexpr int kPeriod = 8 / kRowsPerWindow;  // windows after which the swizzle repeats
+  static constexpr int kStage = 2 * kTileBytes + (kKeys ? (kOneTile ? 512 : kStatsBytes) : 0);
+  static constexpr int kOwn2Ops = 2 * (D / 32) - (kOneTile ? 1 : 0);  // operands of V of 32 owned rows in LDS
+  static constexpr int kOwn2Bytes = kOwn2InLds ? kOwn / 32 * kOwn2Ops * 1024 : 0;
   static constexpr int kSteps0 = 2 * kStage + kOwn2Bytes;  // where a block-sparse list's steps lie
-  static constexpr int kTotal = kSteps0 + (kSteps == 1 ? kListChunk * 8 : 0);
+  static constexpr int kTotal = kSteps0 + (kPaired ? kListChunk * 8 : 0);
 };
 
 // XOR on the 16-byte chunks of LDS row r that keeps both reads of a tile free of bank conflicts (64
@@ -345,12 +355,12 @@ struct Step {
 // Workgroup `wg` of one pass.
 template <int D, typename E, bool kKeys, bool kSparse>
 __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) {
-  using L = BwdLds<D, kKeys>;
+  using L = BwdLds<D, kKeys, kSparse>;
   using V8 = typename E::vec8;
   constexpr int kKC = D / 32;  // MFMA k-steps over d
   constexpr int kDB = D / 16;  // 16-row blocks of the transposed sums
   constexpr bool kHalf = std::is_same<E, Fp16>::value;
-  constexpr bool kPaired = kSparse && L::kSteps == 1;
+  constexpr bool kPaired = L::kPaired, kOneTile = L::kOneTile;
 
   extern __shared__ __align__(16) unsigned char smem[];
   const int tid = threadIdx.x;
@@ -361,6 +371,8 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
 
   const bool split = p.n_split > 1;
   int tile = split ? wg / p.n_split : xcd_remap(wg, p.n_groups, p.xcd_run);
+  const int tile_half = kOneTile ? tile & 1 : 0;
+  if (kOneTile) tile >>= 1;
   if (kSparse && !split && p.order != nullptr) tile = p.order[tile];
   const int ot = tile % p.n_tiles;
   const int bh = tile / p.n_tiles;
@@ -377,7 +389,7 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
   }
   int it0 = 0;  // first streamed tile (dense) of this workgroup's piece
   if (split) {
-    const int piece = wg - tile * p.n_split;
+    const int piece = wg % p.n_split;
     const int first = static_cast<int>(static_cast<int64_t>(n_iter) * piece / p.n_split);
     n_iter = static_cast<int>(static_cast<int64_t>(n_iter) * (piece + 1) / p.n_split) - first;
     if (kSparse)
@@ -385,9 +397,12 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
     else
       it0 = first;
   }
-  const int slot = __builtin_amdgcn_readfirstlane(wave) >> 1;  // the half of the owned rows this wave lies in
-  const int first_row = p.origin + ot * kBM + __builtin_amdgcn_readfirstlane(wave) * 32;
-  const int wbit = first_row < p.own_len && first_row + 31 >= 0 ? 1 << slot : 0;
+  // the half of the owned rows this wave lies in; kOneTile: the half of the streamed rows it takes
+  const int slot = __builtin_amdgcn_readfirstlane(wave) >> 1;
+  const int own_wave = kOneTile ? wave & 1 : wave;
+  const int own_row0 = ot * kBM + tile_half * 64;  // of the grid
+  const int first_row = p.origin + own_row0 + __builtin_amdgcn_readfirstlane(own_wave) * 32;
+  const int wbit = first_row < p.own_len && first_row + 31 >= 0 ? 1 << (kOneTile ? tile_half : slot) : 0;
 
   const float* stats = p.stats + static_cast<int64_t>(bh) * p.stat_blocks * 128;
   // ---- staging, as in the forward: window w of a tile holds LDS bytes [1024 w, +1024) ----
@@ -395,9 +410,10 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
   const u32x4 rsrc2 = raw_rsrc(p.str2.p + b * p.str2.sb + h * p.str2.sh, p.str2_bytes);
   const u32x4 rsrc_st = raw_rsrc(stats, static_cast<uint32_t>(p.stat_blocks) * 512u);
   const uint32_t lds0 = lds_addr(smem);
-  uint32_t src1[L::kWinPerWave], src2[L::kWinPerWave];
+  constexpr int kSrc = L::kPeriod < L::kWinPerWave ? L::kPeriod : L::kWinPerWave;
+  uint32_t src1[kSrc], src2[kSrc];
 #pragma unroll
-  for (int i = 0; i < L::kWinPerWave; ++i) {
+  for (int i = 0; i < kSrc; ++i) {
     const int w = wave * L::kWinPerWave + i;
     const int r = w * L::kRowsPerWindow + (lane * 16) / L::kRowBytes;
     const int ch = (((lane * 16) % L::kRowBytes) / 16) ^ swz<D>(r);
@@ -413,28 +429,27 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
       row = slot == 0 ? x.a * kBN + x.part * 32 : x.b * kBN + x.part * 32 - 32;
 #pragma unroll
     for (int i = 0; i < L::kWinPerWave; ++i)
-      lds_dma16(rsrc1, dst + (wave * L::kWinPerWave + i) * 1024, src1[i] + row * row1, 0);
+      lds_dma16(rsrc1, dst + (wave * L::kWinPerWave + i) * 1024, src1[i % kSrc] + (row + i / kSrc * 8) * row1, 0);
 #pragma unroll
     for (int i = 0; i < L::kWinPerWave; ++i)
-      lds_dma16(rsrc2, dst + L::kTileBytes + (wave * L::kWinPerWave + i) * 1024, src2[i] + row * row2, 0);
+      lds_dma16(rsrc2, dst + L::kTileBytes + (wave * L::kWinPerWave + i) * 1024, src2[i % kSrc] + (row + i / kSrc * 8) * row2, 0);
     if (kKeys && wave == 0) {
       // 16 lanes of -LSE, 16 of -delta, 8 of each per slot; the others load what nobody reads
       uint32_t off = lane * 16 + x.a * 512;
       if (kPaired && x.halves == 0)
         off = ((lane & 8) ? x.b : x.a) * 512 + ((lane & 16) ? 256 : 0) + x.part * 128 + (lane & 7) * 16;
-      lds_dma16(rsrc_st, dst + 2 * L::kTileBytes, off, 0);
+      if (!kOneTile || lane < 32) lds_dma16(rsrc_st, dst + 2 * L::kTileBytes, off, 0);
     }
   };
-  if constexpr (L::kOwn2InLds) {
+  if constexpr (L::kOwn2InLds) {  // operand (rows 16 qq + c16, dims 32 c + 8 g..) of 32 owned rows: 16 bytes a lane
     const int64_t span = (static_cast<int64_t>(p.own_len) - 1) * p.own2.ss * 2 + L::kRowBytes;
     const u32x4 rsrc = raw_rsrc(p.own2.p + b * p.own2.sb + h * p.own2.sh, static_cast<uint32_t>(span));
-#pragma unroll
-    for (int i = 0; i < L::kOwn2Bytes / 1024 / 4; ++i) {
-      const int w = wave * (L::kOwn2Bytes / 1024 / 4) + i;
-      const int r = w * L::kRowsPerWindow + (lane * 16) / L::kRowBytes;
-      const int ch = (((lane * 16) % L::kRowBytes) / 16) ^ swz<D>(r);
-      const uint32_t off = static_cast<uint32_t>(((p.origin + ot * kBM + r) * static_cast<int>(p.own2.ss) + ch * 8) * 2);
-      lds_dma16(rsrc, lds0 + 2 * L::kStage + w * 1024, off, 0);
+    constexpr int kOps = L::kOwn / 32 * L::kOwn2Ops;
+    for (int i = wave; i < kOps; i += 4) {
+      const int o = i % L::kOwn2Ops;
+      const int r = p.origin + own_row0 + i / L::kOwn2Ops * 32 + o / kKC * 16 + c16;
+      const uint32_t off = static_cast<uint32_t>((r * static_cast<int>(p.own2.ss) + (o % kKC) * 32 + 8 * g) * 2);
+      lds_dma16(rsrc, lds0 + 2 * L::kStage + i * 1024, off, 0);
     }
   }
 
@@ -501,12 +516,35 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
       return Step{t, t, j % L::kSteps, rows_bits(e)};
     }
   };
+  // kOneTile: the entries that name this workgroup's keys, 64 of the list at a time
+  const int n_list = __builtin_amdgcn_readfirstlane(n_iter);
+  int chunk = -64, chunk_entry = 0;
+  uint64_t chunk_left = 0;
+  auto next_tile = [&]() -> int {  // or -1
+    while (chunk_left == 0) {
+      chunk += 64;
+      if (chunk >= n_list) return -1;
+      chunk_entry = chunk + lane < n_list ? list[chunk + lane] : 0;
+      const uint64_t named = __ballot(rows_bits(chunk_entry) >> tile_half & 1);
+      chunk_left = static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(named >> 32))) << 32 |
+                   static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(named)));
+    }
+    const int i = __builtin_ctzll(chunk_left);
+    chunk_left &= chunk_left - 1;
+    return __builtin_amdgcn_readlane(chunk_entry, i) >> 2;
+  };
   // the first stage is on its way while the owned rows are read
-  int n_steps = arrange(0);
   Step now{0, 0, 0, 0};
-  if (n_steps > 0) {
-    now = step_at(0);
-    dma(now, 0);
+  int n_steps = 0, now_tile = -1;
+  if constexpr (kOneTile) {
+    now_tile = next_tile();
+    if (now_tile >= 0) dma(Step{now_tile, 0, 0, 3}, 0);
+  } else {
+    n_steps = arrange(0);
+    if (n_steps > 0) {
+      now = step_at(0);
+      dma(now, 0);
+    }
   }
 
   float ds_scale = 1.f;  // fp16: from P (dQ pass) or 2^15 P to 2^e dS
@@ -520,8 +558,8 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
   }
 
   // ---- owned rows (B operands): lane holds row 16qq + c16, dims 32c + 8g.. ----
-  const int row0 = p.origin + ot * kBM + wave * 32 + c16;
-  V8 own1[2][kKC], own2[2][L::kOwn2InLds ? 1 : kKC];
+  const int row0 = p.origin + own_row0 + own_wave * 32 + c16;
+  V8 own1[2][kKC], own2[2][L::kOwn2InLds ? 1 : kKC];  // kOneTile: own2[1][0] is V's last operand
 #pragma unroll
   for (int qq = 0; qq < 2; ++qq) {
     const int row = row0 + 16 * qq;
@@ -532,6 +570,7 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
     for (int i = 0; i < kKC; ++i) {
       own1[qq][i] = as_vec8<V8>(a[4 * i + g]);
       if constexpr (!L::kOwn2InLds) own2[qq][i] = as_vec8<V8>(c[4 * i + g]);
+      if (kOneTile && qq == 1 && i == kKC - 1) own2[1][0] = as_vec8<V8>(c[4 * i + g]);
     }
   }
   float nl_own[2] = {0.f, 0.f}, nd_own[2] = {0.f, 0.f};
@@ -546,24 +585,22 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
   }
 
   // ---- LDS operand addressing ----
+  const uint32_t tile_rows = kOneTile ? slot * 32 * L::kRowBytes : 0;
   uint32_t row_rd[kKC];  // A operand of S and dP: row 16sb + c16, logical chunk 4c + g
 #pragma unroll
   for (int c = 0; c < kKC; ++c)
-    row_rd[c] = pinned(static_cast<uint32_t>(lds0 + c16 * L::kRowBytes + (((4 * c + g) ^ swz<D>(c16)) * 16)));
+    row_rd[c] = pinned(static_cast<uint32_t>(lds0 + tile_rows + c16 * L::kRowBytes + (((4 * c + g) ^ swz<D>(c16)) * 16)));
   // A operand of the sums, transposed: see v_rd in attention.hip
   const int tr_row = 4 * g + (c16 >> 2);
   uint32_t tr_rd[kDB];
 #pragma unroll
   for (int db = 0; db < kDB; ++db) {
     const int d = db * 16 + 4 * (c16 & 3);
-    tr_rd[db] = pinned(static_cast<uint32_t>(lds0 + tr_row * L::kRowBytes + (((d >> 3) ^ swz<D>(tr_row)) * 16) + (d & 7) * 2));
+    tr_rd[db] = pinned(static_cast<uint32_t>(lds0 + tile_rows + tr_row * L::kRowBytes + (((d >> 3) ^ swz<D>(tr_row)) * 16) + (d & 7) * 2));
   }
 
-  const uint32_t stats_rd = pinned(lds0 + 2 * L::kTileBytes + 16 * g);
-  uint32_t own2_rd[L::kOwn2InLds ? kKC : 1];
-  if constexpr (L::kOwn2InLds)
-#pragma unroll
-    for (int c = 0; c < kKC; ++c) own2_rd[c] = pinned(row_rd[c] + 2 * L::kStage + wave * 32 * L::kRowBytes);
+  const uint32_t stats_rd = pinned(lds0 + 2 * L::kTileBytes + 16 * g + (kOneTile ? slot * 128 : 0));
+  const uint32_t own2_rd = pinned(lds0 + 2 * L::kStage + own_wave * L::kOwn2Ops * 1024 + lane * 16);
 
   f32x4 acc1[kDB][2], acc2[kKeys ? kDB : 1][2];
 #pragma unroll
@@ -612,10 +649,12 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
         V8 o[2];
 #pragma unroll
         for (int qq = 0; qq < 2; ++qq) {
-          if constexpr (L::kOwn2InLds)
-            o[qq] = as_vec8<V8>(lds_read16(own2_rd[c] + 16 * qq * L::kRowBytes));
-          else
+          if constexpr (!L::kOwn2InLds)
             o[qq] = own2[qq][c];
+          else if (kOneTile && qq * kKC + c == L::kOwn2Ops)
+            o[qq] = own2[1][0];
+          else
+            o[qq] = as_vec8<V8>(lds_read16(own2_rd + (qq * kKC + c) * 1024));
         }
 #pragma unroll
         for (int sb = 0; sb < 2; ++sb) {
@@ -722,6 +761,7 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
       own1[qq][i] = pinned(own1[qq][i]);
       if constexpr (!L::kOwn2InLds) own2[qq][i] = pinned(own2[qq][i]);
     }
+  if constexpr (kOneTile) own2[1][0] = pinned(own2[1][0]);
   __builtin_amdgcn_s_waitcnt(0);  // V's DMA too, which must not outlive the workgroup
   __syncthreads();
   // A step whose stage is known to the compiler: operand addresses are immediates of its reads.
@@ -745,61 +785,93 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
     __syncthreads();
     now = next;
   };
-  for (int first = 0;;) {
-    for (int j = 0; j < n_steps; j += 2) {
-      run(j, std::integral_constant<int, 0>{});
-      if (j + 1 < n_steps) run(j + 1, std::integral_constant<int, 1>{});
-    }
-    if constexpr (!kPaired) break;
-    first += kListChunk;
-    if (first >= n_iter) break;
-    n_steps = arrange(first);
-    if (n_steps > 0) {
-      now = step_at(0);
-      dma(now, 0);
-    }
+  auto run_tile = [&](auto stage_of_tile) {
+    constexpr int kStageOff = decltype(stage_of_tile)::value * L::kStage;
+    now_tile = next_tile();
+    if (now_tile >= 0) dma(Step{now_tile, 0, 0, 3}, 1 - decltype(stage_of_tile)::value);
+    __builtin_amdgcn_sched_barrier(0);
+    if (wbit) half_tile(kStageOff, kStageOff);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
+  };
+  if constexpr (kOneTile) {
+    while (now_tile >= 0) {
+      run_tile(std::integral_constant<int, 0>{});
+      if (now_tile >= 0) run_tile(std::integral_constant<int, 1>{});
+    }
+  } else {
+    for (int first = 0;;) {
+      for (int j = 0; j < n_steps; j += 2) {
+        run(j, std::integral_constant<int, 0>{});
+        if (j + 1 < n_steps) run(j + 1, std::integral_constant<int, 1>{});
+      }
+      if constexpr (!kPaired) break;
+      first += kListChunk;
+      if (first >= n_iter) break;
+      n_steps = arrange(first);
+      if (n_steps > 0) {
+        now = step_at(0);
+        dma(now, 0);
+      }
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+    }
   }
 
+  // what this wave stores: both sums, or with kOneTile the one that it adds its partner's half to
+  const bool store1 = !kOneTile || slot == 0, store2 = kKeys && (!kOneTile || slot == 1);
+  if constexpr (kOneTile) {
+    f32x4* const at = reinterpret_cast<f32x4*>(smem) + own_wave * 2 * kDB * 2 * 64 + lane;
+    auto put = [&](f32x4 (&acc)[kDB][2], f32x4* to) {
+#pragma unroll
+      for (int db = 0; db < kDB; ++db)
+#pragma unroll
+        for (int qq = 0; qq < 2; ++qq) to[(2 * db + qq) * 64] = acc[db][qq];
+    };
+    auto add = [&](f32x4 (&acc)[kDB][2], const f32x4* from) {
+#pragma unroll
+      for (int db = 0; db < kDB; ++db)
+#pragma unroll
+        for (int qq = 0; qq < 2; ++qq) acc[db][qq] += from[(2 * db + qq) * 64];
+    };
+    if (store1) put(acc2, at + kDB * 2 * 64); else put(acc1, at);
+    __syncthreads();
+    if (store1) add(acc1, at); else add(acc2, at + kDB * 2 * 64);
+  }
+  const float out2_scale = kHalf ? 0x1p-15f : 1.f;
   if (split) {
-    float* part = p.part + static_cast<int64_t>(wg) * (kKeys ? 2 : 1) * kBM * D;
+    const int64_t at = static_cast<int64_t>(tile) * p.n_split + wg % p.n_split;
+    float* part = p.part + at * (kKeys ? 2 : 1) * kBM * D + tile_half * 64 * D;
 #pragma unroll
     for (int qq = 0; qq < 2; ++qq) {
-      float* r = part + (wave * 32 + 16 * qq + c16) * D + 4 * g;
+      float* r = part + (own_wave * 32 + 16 * qq + c16) * D + 4 * g;
 #pragma unroll
       for (int db = 0; db < kDB; ++db) {
-        *reinterpret_cast<f32x4*>(r + db * 16) = acc1[db][qq] * out1_scale;
-        if constexpr (kKeys) *reinterpret_cast<f32x4*>(r + kBM * D + db * 16) = acc2[db][qq] * (kHalf ? 0x1p-15f : 1.f);
+        if (store1) *reinterpret_cast<f32x4*>(r + db * 16) = acc1[db][qq] * out1_scale;
+        if constexpr (kKeys)
+          if (store2) *reinterpret_cast<f32x4*>(r + kBM * D + db * 16) = acc2[db][qq] * out2_scale;
       }
     }
     return;
   }
+  auto store = [&](const f32x4 (&acc)[kDB][2], float scale, uint16_t* out, int64_t ss) {
 #pragma unroll
-  for (int qq = 0; qq < 2; ++qq) {
-    const int row = row0 + 16 * qq;
-    if (row < 0 || row >= p.own_len) continue;
-    uint16_t* o1 = p.out1 + b * p.o1_sb + h * p.o1_sh + row * p.o1_ss;
-#pragma unroll
-    for (int db = 0; db < kDB; ++db) {
-      const f32x4 x = acc1[db][qq] * out1_scale;
-      u32x2 w;
-      w.x = pack2(E::from_float(x[0]), E::from_float(x[1]));
-      w.y = pack2(E::from_float(x[2]), E::from_float(x[3]));
-      *reinterpret_cast<u32x2*>(o1 + db * 16 + 4 * g) = w;
-    }
-    if constexpr (kKeys) {
-      uint16_t* o2 = p.out2 + b * p.o2_sb + h * p.o2_sh + row * p.o2_ss;
+    for (int qq = 0; qq < 2; ++qq) {
+      const int row = row0 + 16 * qq;
+      if (row < 0 || row >= p.own_len) continue;
 #pragma unroll
       for (int db = 0; db < kDB; ++db) {
-        const f32x4 x = acc2[db][qq] * (kHalf ? 0x1p-15f : 1.f);
+        const f32x4 x = acc[db][qq] * scale;
         u32x2 w;
         w.x = pack2(E::from_float(x[0]), E::from_float(x[1]));
         w.y = pack2(E::from_float(x[2]), E::from_float(x[3]));
-        *reinterpret_cast<u32x2*>(o2 + db * 16 + 4 * g) = w;
+        *reinterpret_cast<u32x2*>(out + row * ss + db * 16 + 4 * g) = w;
       }
     }
-  }
+  };
+  if (store1) store(acc1, out1_scale, p.out1 + b * p.o1_sb + h * p.o1_sh, p.o1_ss);
+  if constexpr (kKeys)
+    if (store2) store(acc2, out2_scale, p.out2 + b * p.o2_sb + h * p.o2_sh, p.o2_ss);
 }
 
 // Waves per SIMD that the registers are held to.
@@ -945,8 +1017,9 @@ __global__ __launch_bounds__(1024) void order_kernel(OrderParams p) {
 }
 
 template <int D, typename E, bool kSparse>
-int launch_passes(const BothPasses& p, hipStream_t st) {
-  constexpr int kLds = BwdLds<D, true>::kTotal > BwdLds<D, false>::kTotal ? BwdLds<D, true>::kTotal : BwdLds<D, false>::kTotal;
+int launch_passes(const BothPasses& p, int batch, hipStream_t st) {
+  constexpr int kLdsKeys = BwdLds<D, true, kSparse>::kTotal, kLdsRows = BwdLds<D, false, kSparse>::kTotal;
+  constexpr int kLds = kLdsKeys > kLdsRows ? kLdsKeys : kLdsRows;
   auto kernel = attention_bwd_kernel<D, E, kSparse>;
   static LaunchSetup once;
   if (set_dynamic_lds_once(once, reinterpret_cast<const void*>(kernel), kLds) != hipSuccess) {
@@ -956,7 +1029,7 @@ int launch_passes(const BothPasses& p, hipStream_t st) {
   const int last_dq = p.first_dq + p.dq.n_groups, last_dkv = p.first_dkv + p.dkv.n_groups;
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(last_dq > last_dkv ? last_dq : last_dkv)), dim3(kThreads), kLds, st, p);
   MODDIT_CHECK_LAUNCH("attention_bwd");
-  auto combined = [](const BwdParams& q) { return q.n_split > 1 ? q.n_groups / q.n_split * (kBM / kCombineRows) : 0; };
+  auto combined = [&](const BwdParams& q) { return q.n_split > 1 ? batch * q.heads * q.n_tiles * (kBM / kCombineRows) : 0; };
   const int first_dq = 2 * combined(p.dkv), groups = first_dq + combined(p.dq);
   if (groups > 0) {
     hipLaunchKernelGGL((combine_bwd_kernel<D, E>), dim3(groups), dim3(kThreads), 0, st, p, first_dq);
@@ -988,7 +1061,7 @@ int launch_bwd(const StatsParams& sp, const BothPasses& p, int batch, hipStream_
     hipLaunchKernelGGL(order_kernel, dim3(2), dim3(1024), 0, st, op);
     MODDIT_CHECK_LAUNCH("attention_bwd (order)");
   }
-  return dq.counts != nullptr ? launch_passes<D, E, true>(p, st) : launch_passes<D, E, false>(p, st);
+  return dq.counts != nullptr ? launch_passes<D, E, true>(p, batch, st) : launch_passes<D, E, false>(p, batch, st);
 }
 
 // ---- sizes ----
@@ -1224,6 +1297,7 @@ int bwd_entry(const BwdArgs& a, moddit_stream_t stream) {
 
   dq.n_groups = static_cast<int>(plan.tiles[0] * a.batch * a.heads * plan.n_split[0]);
   dkv.n_groups = static_cast<int>(plan.tiles[1] * a.batch * a.heads * plan.n_split[1]);
+  if (lists && a.head_dim == 128) dkv.n_groups *= 2;  // BwdLds::kOneTile
   const int first = ((plan.dq_first ? dq : dkv).n_groups + kNumXcd - 1) / kNumXcd * kNumXcd;
   const BothPasses both{dkv, dq, plan.dq_first ? first : 0, plan.dq_first ? 0 : first};
   hipStream_t st = as_stream(stream);

@@ -37,7 +37,7 @@ namespace {
 constexpr int kBM = 128;  // owned rows per workgroup
 constexpr int kBN = 64;   // streamed rows per tile
 constexpr int kThreads = 256;
-constexpr int kStatsBytes = 1024;  // one DMA window; a block's 64 -LSE and 64 -delta take half
+constexpr int kStatsBytes = 512;  // a block's 64 -LSE and 64 -delta
 constexpr float kPExponent = 15.f;  // fp16: P is held as 2^15 P
 constexpr int kFewKeys = 64;
 
@@ -57,25 +57,29 @@ constexpr int kListChunk = 2 * kThreads;
 // At D = 128 the dK/dV pass has no registers for V beside its sums (128) and K (32): V stays in LDS,
 // as MFMA operands of 1 KB, and stages are half a tile so that two workgroups fit a CU.
 //
-// Its block-sparse form owns one 64-key tile (kOneTile): an entry of a list by 128 keys names both
-// halves of the keys less than half the time (random masks), and waves of the other half would wait.
-// Two waves take the first 32 rows of each streamed tile and two the others, with sums that are added
-// at the end. One operand of V a wave is held in registers so that this fits 80 KB.
+// The block-sparse dK/dV pass owns one 64-key tile (kOneTile): an entry of a list by 128 keys often
+// names one half of them (61 % of a random mask's entries), and the waves of the other would wait. Two
+// waves take the first 32 rows of each streamed tile and two the others, with sums that are added at
+// the end. 64x64 blocks: 28,800 tokens x 12 heads, D = 128 3.48 -> 3.23 ms, 7,680 x 12 487 -> 435 us,
+// 17,776 x 16, D = 64 1.65 -> 1.55 ms; where entries name both halves (128x128 blocks, nearly full
+// masks) the streamed rows that are read twice cost 5 %. At D = 128 one operand of V a wave is held in
+// registers, so that this fits 80 KB.
 template <int D, bool kKeys, bool kSparse>
 struct BwdLds {
   static constexpr bool kOwn2InLds = kKeys && D == 128;
-  static constexpr bool kOneTile = kOwn2InLds && kSparse;
+  static constexpr bool kOneTile = kKeys && kSparse;
+  static constexpr bool kOwn2Kept = kOneTile && kOwn2InLds;
+  static constexpr bool kPaired = !kKeys && kSparse;   // see Step
   static constexpr int kOwn = kOneTile ? 64 : kBM;     // owned rows
   static constexpr int kRows = kOwn2InLds && !kOneTile ? 32 : kBN;  // streamed rows of a stage
   static constexpr int kSteps = kBN / kRows;           // stages of a tile
-  static constexpr bool kPaired = kSparse && kSteps == 1 && !kOneTile;  // see Step
   static constexpr int kRowBytes = D * 2;
   static constexpr int kTileBytes = kRows * kRowBytes;  // one tensor's part of a stage
   static constexpr int kRowsPerWindow = 1024 / kRowBytes;
   static constexpr int kWinPerWave = kTileBytes / 1024 / 4;
   static constexpr int kPeriod = 8 / kRowsPerWindow;  // windows after which the swizzle repeats
-  static constexpr int kStage = 2 * kTileBytes + (kKeys ? (kOneTile ? 512 : kStatsBytes) : 0);
-  static constexpr int kOwn2Ops = 2 * (D / 32) - (kOneTile ? 1 : 0);  // operands of V of 32 owned rows in LDS
+  static constexpr int kStage = 2 * kTileBytes + (kKeys ? kStatsBytes : 0);
+  static constexpr int kOwn2Ops = 2 * (D / 32) - (kOwn2Kept ? 1 : 0);  // operands of V of 32 owned rows in LDS
   static constexpr int kOwn2Bytes = kOwn2InLds ? kOwn / 32 * kOwn2Ops * 1024 : 0;
   static constexpr int kSteps0 = 2 * kStage + kOwn2Bytes;  // where a block-sparse list's steps lie
   static constexpr int kTotal = kSteps0 + (kPaired ? kListChunk * 8 : 0);
@@ -341,13 +345,13 @@ __device__ __forceinline__ int ds_exponent(const float* maxima, int n, float (*r
   return e < -100 ? -100 : (e > 100 ? 100 : e);
 }
 
-// What a stage holds and who computes on it. With kSteps == 1 a stage has two slots of 32 rows: the
-// halves of tile a, for the halves of the owned rows whose bits are set in `halves`; or, with none
-// set, half `part` of tile a for the first half of the owned rows and of tile b for the second: list
+// What a stage holds and who computes on it. In the block-sparse dQ pass a stage has two slots of 32
+// rows: the halves of tile a, for the halves of the owned rows whose bits are set in `halves`; or, with
+// none set, half `part` of tile a for the first half of the owned rows and of tile b for the second: list
 // entries that one half uses go in pairs, and neither half waits while the other works (random masks:
-// 17,776 tokens x 16 heads, D = 64 1.84 -> 1.76 ms; 7,680 x 12, D = 128, where only the dQ pass has them,
-// 521 -> 493 us). With kSteps == 2 a stage is half `part` of tile a: two slots of 32 rows would not fit
-// beside V with two workgroups to a CU.
+// 17,776 tokens x 16 heads, D = 64, both passes 1.84 -> 1.76 ms; 7,680 x 12, D = 128 521 -> 493 us).
+// Owning one 64-row tile here too is 1 % slower on 64x64 blocks and 3 to 6 % on others.
+// With kSteps == 2 a stage is half `part` of tile a.
 struct Step {
   int a, b, part, halves;
 };
@@ -433,13 +437,7 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
 #pragma unroll
     for (int i = 0; i < L::kWinPerWave; ++i)
       lds_dma16(rsrc2, dst + L::kTileBytes + (wave * L::kWinPerWave + i) * 1024, src2[i % kSrc] + (row + i / kSrc * 8) * row2, 0);
-    if (kKeys && wave == 0) {
-      // 16 lanes of -LSE, 16 of -delta, 8 of each per slot; the others load what nobody reads
-      uint32_t off = lane * 16 + x.a * 512;
-      if (kPaired && x.halves == 0)
-        off = ((lane & 8) ? x.b : x.a) * 512 + ((lane & 16) ? 256 : 0) + x.part * 128 + (lane & 7) * 16;
-      if (!kOneTile || lane < 32) lds_dma16(rsrc_st, dst + 2 * L::kTileBytes, off, 0);
-    }
+    if (kKeys && wave == 0 && lane < 32) lds_dma16(rsrc_st, dst + 2 * L::kTileBytes, lane * 16 + x.a * kStatsBytes, 0);
   };
   if constexpr (L::kOwn2InLds) {  // operand (rows 16 qq + c16, dims 32 c + 8 g..) of 32 owned rows: 16 bytes a lane
     const int64_t span = (static_cast<int64_t>(p.own_len) - 1) * p.own2.ss * 2 + L::kRowBytes;
@@ -570,14 +568,14 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
     for (int i = 0; i < kKC; ++i) {
       own1[qq][i] = as_vec8<V8>(a[4 * i + g]);
       if constexpr (!L::kOwn2InLds) own2[qq][i] = as_vec8<V8>(c[4 * i + g]);
-      if (kOneTile && qq == 1 && i == kKC - 1) own2[1][0] = as_vec8<V8>(c[4 * i + g]);
+      if (L::kOwn2Kept && qq == 1 && i == kKC - 1) own2[1][0] = as_vec8<V8>(c[4 * i + g]);
     }
   }
   float nl_own[2] = {0.f, 0.f}, nd_own[2] = {0.f, 0.f};
   if constexpr (!kKeys) {
 #pragma unroll
     for (int qq = 0; qq < 2; ++qq) {
-      const int gr = ot * kBM + wave * 32 + 16 * qq + c16;
+      const int gr = own_row0 + own_wave * 32 + 16 * qq + c16;
       const float* s = stats + (gr >> 6) * 128 + (gr & 63);
       nl_own[qq] = s[0] - (kHalf ? kPExponent : 0.f);
       nd_own[qq] = s[64];
@@ -651,7 +649,7 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
         for (int qq = 0; qq < 2; ++qq) {
           if constexpr (!L::kOwn2InLds)
             o[qq] = own2[qq][c];
-          else if (kOneTile && qq * kKC + c == L::kOwn2Ops)
+          else if (L::kOwn2Kept && qq * kKC + c == L::kOwn2Ops)
             o[qq] = own2[1][0];
           else
             o[qq] = as_vec8<V8>(lds_read16(own2_rd + (qq * kKC + c) * 1024));
@@ -761,7 +759,7 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
       own1[qq][i] = pinned(own1[qq][i]);
       if constexpr (!L::kOwn2InLds) own2[qq][i] = pinned(own2[qq][i]);
     }
-  if constexpr (kOneTile) own2[1][0] = pinned(own2[1][0]);
+  if constexpr (L::kOwn2Kept) own2[1][0] = pinned(own2[1][0]);
   __builtin_amdgcn_s_waitcnt(0);  // V's DMA too, which must not outlive the workgroup
   __syncthreads();
   // A step whose stage is known to the compiler: operand addresses are immediates of its reads.
@@ -818,11 +816,11 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
     }
   }
 
-  // what this wave stores: both sums, or with kOneTile the one that it adds its partner's half to
+  // what this wave stores: all its sums, or with kOneTile the one that it adds its partner's half to
   const bool store1 = !kOneTile || slot == 0, store2 = kKeys && (!kOneTile || slot == 1);
   if constexpr (kOneTile) {
     f32x4* const at = reinterpret_cast<f32x4*>(smem) + own_wave * 2 * kDB * 2 * 64 + lane;
-    auto put = [&](f32x4 (&acc)[kDB][2], f32x4* to) {
+    auto put = [&](const f32x4 (&acc)[kDB][2], f32x4* to) {
 #pragma unroll
       for (int db = 0; db < kDB; ++db)
 #pragma unroll
@@ -1105,10 +1103,11 @@ BwdPlan plan_bwd(int batch, int heads, int q_len, int kv_len, int head_dim, int 
   // adding fp32 partial sums and one more launch (5 us). 256 rows x 29,019 keys x 24 heads, D = 128:
   // 1,240 us without, 440 with; 4,096 tokens x 2 heads, D = 64: 178 and 73.
   double all_us = 0.0, piece_us[2];
-  for (int i = 0; i < 2; ++i) all_us += bh * p.tiles[i] * (steps[i] + kFixedSteps) * step_us(head_dim, i == 1);
+  const double halves[2] = {1.0, cap > 0 ? 2.0 : 1.0};  // workgroups of a tile (BwdLds::kOneTile)
+  for (int i = 0; i < 2; ++i) all_us += bh * p.tiles[i] * (steps[i] + halves[i] * kFixedSteps) * step_us(head_dim, i == 1);
   all_us /= resident(head_dim);
   for (int i = 0; i < 2; ++i) {
-    const double sweep_us = steps[i] * step_us(head_dim, i == 1);
+    const double sweep_us = steps[i] * step_us(head_dim, i == 1) / halves[i];
     int64_t n = 1;
     if (sweep_us > all_us + 10.0) {
       n = static_cast<int64_t>(std::ceil(sweep_us / all_us));
@@ -1297,7 +1296,7 @@ int bwd_entry(const BwdArgs& a, moddit_stream_t stream) {
 
   dq.n_groups = static_cast<int>(plan.tiles[0] * a.batch * a.heads * plan.n_split[0]);
   dkv.n_groups = static_cast<int>(plan.tiles[1] * a.batch * a.heads * plan.n_split[1]);
-  if (lists && a.head_dim == 128) dkv.n_groups *= 2;  // BwdLds::kOneTile
+  if (lists) dkv.n_groups *= 2;  // BwdLds::kOneTile
   const int first = ((plan.dq_first ? dq : dkv).n_groups + kNumXcd - 1) / kNumXcd * kNumXcd;
   const BothPasses both{dkv, dq, plan.dq_first ? first : 0, plan.dq_first ? 0 : first};
   hipStream_t st = as_stream(stream);

@@ -856,14 +856,22 @@ __device__ __forceinline__ void bwd_workgroup(const BwdParams& p, const int wg) 
 #pragma unroll
     for (int qq = 0; qq < 2; ++qq) {
       const int row = row0 + 16 * qq;
-      if (row < 0 || row >= p.own_len) continue;
+      const bool in = row >= 0 && row < p.own_len;
+      uint16_t* const at = out + row * ss;
+      // lanes g and g + 1 trade halves of two blocks of 16 dims: 16 bytes a lane, 64 of a row (32 of a row
+      // at a time: 256 rows x 29,019 keys x 24 heads 381 -> 367 us)
 #pragma unroll
-      for (int db = 0; db < kDB; ++db) {
-        const f32x4 x = acc[db][qq] * scale;
-        u32x2 w;
-        w.x = pack2(E::from_float(x[0]), E::from_float(x[1]));
-        w.y = pack2(E::from_float(x[2]), E::from_float(x[3]));
-        *reinterpret_cast<u32x2*>(out + row * ss + db * 16 + 4 * g) = w;
+      for (int db = 0; db < kDB; db += 2) {
+        u32x2 w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const f32x4 x = acc[db + i][qq] * scale;
+          w[i].x = pack2(E::from_float(x[0]), E::from_float(x[1]));
+          w[i].y = pack2(E::from_float(x[2]), E::from_float(x[3]));
+        }
+        const auto x = __builtin_amdgcn_permlane16_swap(w[0].x, w[1].x, false, false);
+        const auto y = __builtin_amdgcn_permlane16_swap(w[0].y, w[1].y, false, false);
+        if (in) *reinterpret_cast<u32x4*>(at + (db + (g & 1)) * 16 + 4 * (g & 2)) = u32x4{x[0], y[0], x[1], y[1]};
       }
     }
   };

@@ -7,12 +7,17 @@
 // A (row, key) pair takes 10 D FLOP. P is computed again from Q, K and the LSE: nothing of the
 // size of P is kept.
 //
-// Two passes of one kernel body, in one launch. Each workgroup owns 128 rows of one side and streams tiles of 64
-// rows of the other: the dQ pass owns queries and streams keys, the dK/dV pass owns keys and
-// streams queries, so every sum stays in one workgroup's registers: no atomics, and results do
+// Two passes of one kernel body, in one launch. Each workgroup owns 128 rows of one side and streams
+// tiles of 64 rows of the other: the dQ pass owns queries and streams keys, the dK/dV pass owns keys
+// and streams queries, so every sum stays in one workgroup's registers: no atomics, and results do
 // not depend on the order of workgroups. The price is that S and dP are computed twice, 14 D FLOP
 // a pair; adding dQ's parts across workgroups instead would take 4 D bytes of atomics per row and
 // 128 keys, more time than the products (2 D 128 FLOP each), in an order that changes.
+//
+// Bound by the matrix cores: 29,019 tokens x 12 heads, D = 128 in 13.4 to 13.9 ms, 1.3 PFLOP/s of the
+// 14 D at the board's power limit (926 to 965 TFLOP/s of the 10 D asked for). At D = 64 the weights
+// take nearly as many VALU cycles as the products take of the matrix cores: 1,577 x 48 heads in
+// 109 us, 0.98 PFLOP/s of the 14 D.
 //
 // As in the forward the products are transposed: streamed rows are the A operand and owned rows
 // the columns, on MFMA 16x16x32. The accumulators of S and dP (streamed 4g + j, owned c16) are
@@ -21,8 +26,8 @@
 // ds_read_b64_tr_b16.
 //
 // Rows of the grid outside the sequence: streamed ones load zeros; as queries they have
-// -LSE = -inf, so P = 0, as keys their scores are set to -inf. A query without keys has LSE = -inf
-// and adds nothing. Owned ones load a clamped row and store nothing.
+// -LSE = -inf, so P = 0, as keys their P, at most 1, meets zeros of K. A query without keys has
+// LSE = -inf and adds nothing. Owned ones load a clamped row and store nothing.
 //
 // fp16 holds 2^-24 to 65504: P is rounded as 2^15 P, and dS as 2^e dS with the largest e for
 // which the head's largest |dO| (|V| + |O|) + |dL| stays below 2^14; bf16 needs neither.
@@ -165,7 +170,7 @@ struct StatsParams {
 
 // Block i of a head: -LSE (log2 units, with the exponent that P is held at) and -delta of the 64
 // grid rows from 64 i on; with kMax also the largest finite |dO|^2, |O|^2, |V|^2 and |dL| of its rows.
-// Reads O, dO (and V) once: bound by HBM.
+// Reads O, dO (and V) once: bound by HBM (29,019 tokens x 12 heads, D = 128: 36 us, 5.0 TB/s).
 //
 // The softmax over one key is 1 whatever its score: dP = delta, and dS = P dL exactly. The rounding of
 // O and of the sums would leave a remainder, so delta keeps -dL alone there and the passes see a zero V.
@@ -902,7 +907,7 @@ __global__ __launch_bounds__(kThreads, bwd_waves(D)) __attribute__((amdgpu_waves
 
 // The pieces of a tile -> its rows, added in piece order. A workgroup takes kCombineRows rows of
 // one tile and tensor, a thread four of its columns. Bound by reading the partials back, mostly
-// from L2 and the last-level cache.
+// from L2 and the last-level cache (4,096 tokens x 2 heads, D = 64: 40 MB in 7.7 us).
 constexpr int kCombineRows = 16;
 
 template <int D, typename E>
@@ -940,7 +945,8 @@ __global__ __launch_bounds__(kThreads) void combine_bwd_kernel(BothPasses both, 
 // A full column of a mask (text keys, a kept line) gives a key tile many times the mean of
 // queries; started last, it runs alone at the end. The tiles of each pass in order of how far
 // their lists lie above the mean, kept in their natural order within a class, so that neighbours
-// still share what they stream. One workgroup per pass.
+// still share what they stream. One workgroup per pass: 8 us, of which 28,800 tokens x 12 heads
+// gain 220 (3.69 -> 3.47 ms).
 struct OrderParams {
   const int32_t* counts[2];
   int32_t* order[2];
@@ -1318,7 +1324,7 @@ int bwd_entry(const BwdArgs& a, moddit_stream_t stream) {
 // Workgroup (head, 16 key tiles of 128): the bits (query block of 64 rows, key tile of 64) of its
 // 32 key tiles are set in LDS by threads that each walk their query tiles' lists (ascending, so a
 // binary search finds the part inside), then each wave writes the list of four key tile pairs,
-// 64 query blocks at a time.
+// 64 query blocks at a time. Latency of the walks: 28,800 tokens x 12 heads, 19 % of the blocks, 19 us.
 constexpr int kPairs = 16;
 constexpr int kMaxBlocks = 12288;  // query blocks a call: 32 rows of bits in 48 KB of LDS
 

@@ -165,7 +165,8 @@ __device__ __forceinline__ void turn(float (&x)[8], const float (&c)[4], const f
 // ---- norm over a head's D (or none) ----
 // A wave's item is 64 / (D/8) rows at a time: heads of one token where those lie next to each
 // other, else tokens of one head; it walks its heads, kUnroll at a time with the loads of q and
-// k in flight together, so that a token's angles are read once.
+// k in flight together, so that a token's angles are read once. 115,200 tokens x 24 heads, D = 128,
+// RMS, bf16: 534 us, 5.4 TB/s; gradient of 17,776 x 48, D = 64, layer norm, fp16: 155 us, 4.2 TB/s.
 template <int D, typename E, int kNorm, bool kInter, bool kBwd>
 __global__ __launch_bounds__(kThreads) void norm_rope_heads_kernel(RopeParams p) {
   constexpr int kLanes = D / 8;
@@ -304,7 +305,8 @@ __global__ __launch_bounds__(kThreads) void norm_rope_heads_kernel(RopeParams p)
 // ---- norm over all heads of a token, forward ----
 // One wave per token and tensor at a time, all its loads (kChunks of 16 bytes a lane) in flight
 // together and no barrier; the weights wait in LDS as fp32, in two halves of 16 bytes a group of
-// 8 elements so that a wave's reads are contiguous.
+// 8 elements so that a wave's reads are contiguous. 69,120 tokens x 40 heads, D = 128: 565 us, 5.1 TB/s
+// (a workgroup per token, whose sums wait at a barrier: 1,390).
 template <int kChunks, typename E, int kNorm, bool kInter, bool kBias>
 __global__ __launch_bounds__(kThreads) void norm_rope_wave_kernel(RopeParams p) {
   extern __shared__ float affine[];  // [w, bias][2][n_chunks][4]
@@ -392,7 +394,8 @@ __global__ __launch_bounds__(kThreads) void norm_rope_wave_kernel(RopeParams p) 
 // One workgroup per token and tensor at a time; a thread holds kChunks groups of 8 elements, all at
 // the same place of their heads (the workgroup's size is a multiple of a row's lanes), and their
 // weights across tokens. The next token's rows are loaded before the sums of the current one,
-// which wait at a barrier.
+// which wait at a barrier. 28,800 tokens x 40 heads, D = 128: 440 us, 4.0 TB/s, two workgroups a CU by
+// registers; a wave per token spills (742 us and more).
 template <int kChunks, typename E, int kNorm, bool kInter, bool kBias>
 __global__ __launch_bounds__(kThreads) void norm_rope_token_bwd_kernel(RopeParams p) {
   const int which = blockIdx.y;
@@ -531,7 +534,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_token_bwd_kernel(RopeParam
 }
 
 // Sums over the workgroups' records, in 64 bits and in a fixed order: 64 columns per workgroup,
-// the records dealt to its waves.
+// the records dealt to its waves: 768 records of 5,120 values, q and k, in 8 us.
 struct SumParams {
   const float* partial;
   float* out[4];
@@ -568,7 +571,8 @@ __global__ __launch_bounds__(1024) void norm_rope_sum_kernel(SumParams p) {
 
 // ---- host side ----
 // Workgroups of a backward call, each of which leaves a record of partial sums: enough to fill
-// the card, few enough that the records stay small beside the tensors.
+// the card, few enough that the records stay small beside the tensors (over all heads 1,536 records
+// instead of 768: 527 us in place of 503, 28,800 tokens x 40 heads).
 int backward_groups(int64_t work_groups, int across) {
   const int64_t most = across ? 768 : 1536;
   return static_cast<int>(work_groups < 1 ? 1 : (work_groups < most ? work_groups : most));

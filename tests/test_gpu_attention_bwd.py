@@ -166,6 +166,22 @@ def test_lists_of_many_entries(D, dtype, rows, keys):
     _run(q, k, v, do, mask=mask, tiles=tiles)
 
 
+@pytest.mark.parametrize("D,dtype", [(64, BF), (128, FP)])
+@pytest.mark.parametrize("rows,keys,batch", [(190, 70 * 640, 24), (70 * 640, 150, 40)])
+def test_lists_of_many_entries_on_a_full_card(D, dtype, rows, keys, batch):
+    """The same with so many workgroups that none shares its list: every batch has the first's result."""
+    g = torch.Generator().manual_seed(6)
+    m = (torch.rand((1, -(-rows // 64), -(-keys // 64)), generator=g) < 0.6).cuda()
+    tiles = ops.mask_to_tiles(m, 64, union_rows=False)
+    q, k, v, do = _tensors(1, 1, rows, keys, D, dtype, False)
+    mask = m.repeat_interleave(64, 1).repeat_interleave(64, 2)[None, :, :rows, :keys]
+    out, lse, grads, tol = _ref(q, k, v, do, D ** -0.5, mask)
+    many = [t.expand(batch, *t.shape[1:]) for t in (q, k, v, out.to(dtype), lse.float(), do)]
+    got = ops.block_sparse_bwd(*many, tiles)
+    _check([t[:1] for t in got], grads, tol, dtype)
+    assert all(torch.equal(t, t[:1].expand_as(t)) for t in got)
+
+
 @pytest.mark.parametrize("H,nq,nk,p", [(1, 1, 1, 1.0), (2, 5, 3, 0.5), (3, 40, 70, 0.1), (1, 7, 33, 0.0), (2, 130, 64, 0.9)])
 def test_transpose_tiles(H, nq, nk, p):
     """Every (query block, key tile) pair of the lists, and no other, in ascending order."""
@@ -399,6 +415,34 @@ def test_a_training_step_of_a_layer(sparse, dtype):
     dq, dk, dwq, dwk, _, _ = ops.qk_norm_rope_bwd(q, k, da, db, **kw)
     for x, want in zip(got, (dq, dk, dv, dwq, dwk)):
         assert torch.equal(x, want)
+
+
+def test_a_training_step_in_a_graph():
+    """Forward and backward of a layer on leaves of their own, captured and replayed."""
+    q, k, v, w, cos, sin = _layer(1, 2, 200, 64, BF, 3)
+    dy = torch.randn_like(q)
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, *w)]
+        a, b = md.qk_norm_rope(leaves[0], leaves[1], q_weight=leaves[3], k_weight=leaves[4], cos=cos, sin=sin)
+        return torch.autograd.grad(md.flash_attention(a, b, leaves[2]), leaves, dy)
+
+    want = [t.clone() for t in step()]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    for _ in range(3):
+        for t in got:
+            t.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert all(torch.equal(a, b) for a, b in zip(step(), want))
 
 
 def test_autograd_edges():

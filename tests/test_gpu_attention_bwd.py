@@ -199,6 +199,38 @@ def test_transpose_tiles(H, nq, nk, p):
             assert got.entries[h, t, :n].tolist() == want
 
 
+def test_a_large_layer():
+    """A HunyuanVideo-like layer, 24 heads of 115,163 tokens, 17 % of the blocks: sampled rows of dQ and
+    of dK and dV. out and lse are the forward's own, so that their rounding is part of the formula."""
+    H, S, D, scale, u = 24, 115163, 128, 128 ** -0.5, 2.0 ** -8
+    g = torch.Generator("cuda").manual_seed(7)
+    q, k, v, do = (torch.randn((1, S, H, D), generator=g, device="cuda").to(BF).transpose(1, 2) for _ in range(4))
+    m = torch.rand((H, 1800, 1800), generator=g, device="cuda") < 0.17
+    m[:, :, 700] = True
+    tiles = ops.mask_to_tiles(m, 64, union_rows=False)
+    out, lse = ops.block_sparse_fwd(q, k, v, tiles, return_lse=True)
+    got = ops.block_sparse_bwd(q, k, v, out, lse, do, tiles)
+    for h in (0, 11, 23):
+        Q, K, V, dO, L = (t[0, h].double() for t in (q, k, v, do, lse))
+        C = (dO * out[0, h].double()).abs().sum(-1)
+        delta = (dO * out[0, h].double()).sum(-1)
+        pick = torch.tensor([0, 63, 64, 127, 44800, 44863, 60001, 115100, S - 1], device="cuda")
+        allowed = m[h][pick // 64].repeat_interleave(64, 1)[:, :S]
+        p = torch.exp(Q[pick] @ K.T * scale - L[pick, None]).masked_fill(~allowed, 0.0)
+        ds = p * (dO[pick] @ V.T - delta[pick, None])
+        err = (u + 2.0 ** -14 + 2.0 ** -17) * ds.abs() + p * 2.0 ** -17 * (dO[pick].abs() @ V.abs().T + C[pick, None])
+        want, tol = scale * ds @ K, scale * err @ K.abs()
+        assert ((got[0][0, h, pick].double() - want).abs() <= tol + u * want.abs() + 2.0 ** -25).all()
+        allowed = m[h][:, pick // 64].repeat_interleave(64, 0)[:S]
+        p = torch.exp(Q @ K[pick].T * scale - L[:, None]).masked_fill(~allowed, 0.0)
+        ds = p * (dO @ V[pick].T - delta[:, None])
+        err = (u + 2.0 ** -14 + 2.0 ** -17) * ds.abs() + p * 2.0 ** -17 * (dO.abs() @ V[pick].abs().T + C[:, None])
+        want, tol = scale * ds.T @ Q, scale * err.T @ Q.abs()
+        assert ((got[1][0, h, pick].double() - want).abs() <= tol + u * want.abs() + 2.0 ** -25).all()
+        want, tol = p.T @ dO, (u + 2.0 ** -14 + 2.0 ** -17) * p.T @ dO.abs()
+        assert ((got[2][0, h, pick].double() - want).abs() <= tol + u * want.abs() + 2.0 ** -25).all()
+
+
 def test_entries_past_the_last_tile():
     """A 128-token mask whose last block the sequence half fills lists a key tile past the end."""
     m = torch.ones((1, 3, 3), dtype=torch.bool, device="cuda")

@@ -226,8 +226,8 @@ _MAX_QTILES = 6144  # query tiles whose transposed bits fit a workgroup's LDS
 
 
 def transpose_tiles(tiles: TileList, kv_len: int) -> KeyTileList:
-    """The KeyTileList of `tiles`, whose entries ascend (`mask_to_tiles`), for kv_len keys. A program that trains under one mask for several
-    calls keeps it and hands it to `block_sparse_bwd`."""
+    """The KeyTileList of `tiles`, whose entries ascend (`mask_to_tiles`), for kv_len keys. A program
+    that trains under one mask for several calls keeps it and hands it to `block_sparse_bwd`."""
     _require_gpu(tiles.counts, tiles.entries, what="transpose_tiles")
     H, nq = tiles.counts.shape
     if kv_len < 0:
